@@ -34,6 +34,68 @@ std::vector<at::Tensor> ce_fwd_bwd(at::Tensor& logits, const at::Tensor& target,
   return {loss, lse};
 }
 
+// ---- token log probabilities (token_logprobs.hip) -----------------------------------------------
+struct LogitRows {
+  int64_t rows, s0, s1;
+  int inner, V;
+};
+
+// logits [V], [R, V] or [B, S, V] with unit stride in V (any strides in the others)
+LogitRows logit_rows(const at::Tensor& z, const at::Tensor& target, const char* who) {
+  HYP_CHECK_CUDA_TENSOR(z);
+  const int d = (int)z.dim();
+  TORCH_CHECK(d >= 1 && d <= 3 && z.size(-1) >= 1 && z.size(-1) < (int64_t)INT32_MAX && (z.stride(-1) == 1 || z.size(-1) == 1),
+              who, ": logits must be [V], [R, V] or [B, S, V] with unit stride in V >= 1");
+  LogitRows r;
+  r.V = (int)z.size(-1);
+  const int64_t inner = d >= 2 ? z.size(d - 2) : 1;
+  r.rows = z.numel() / r.V;
+  r.s1 = d >= 2 ? z.stride(d - 2) : 0;
+  r.s0 = d == 3 ? z.stride(0) : 0;
+  TORCH_CHECK(r.rows < hyp::kTokenRowsMax, who, ": at most 2^24 - 1 rows");
+  r.inner = (int)std::max<int64_t>(1, inner);
+  TORCH_CHECK(target.scalar_type() == at::kLong && target.is_contiguous() && target.numel() == r.rows &&
+                  target.device() == z.device(),
+              who, ": target must be a contiguous int64 tensor with one id for each row, on the logits' device");
+  return r;
+}
+
+// (logprobs, entropy, stats [rows, 3], top logprobs [rows, k], top ids [rows, k])
+std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& z, const at::Tensor& target, int64_t k, int64_t ignore_index,
+                                           double inv_t) {
+  const LogitRows r = logit_rows(z, target, "token_logprobs_fwd");
+  TORCH_CHECK(k >= 0 && k <= hyp::kTokenTopMax && k <= r.V, "token_logprobs_fwd: k must be in [0, min(V, ",
+              hyp::kTokenTopMax, ")]");
+  const at::DeviceGuard guard(z.device());
+  auto fopt = z.options().dtype(at::kFloat);
+  auto lp = at::empty({r.rows}, fopt), ent = at::empty({r.rows}, fopt), stats = at::empty({r.rows, 3}, fopt);
+  auto tl = at::empty({r.rows, k}, fopt), ti = at::empty({r.rows, k}, z.options().dtype(at::kLong));
+  HYP_CHECK_HIP(hyp::token_logprobs_fwd(dtype_code(z), z.data_ptr(), r.s0, r.s1, r.inner, r.rows, r.V,
+                                        target.data_ptr<int64_t>(), ignore_index, (float)inv_t, lp.data_ptr<float>(),
+                                        ent.data_ptr<float>(), stats.data_ptr<float>(), (int)k, tl.data_ptr<float>(),
+                                        ti.data_ptr<int64_t>(), cur_stream()));
+  return {lp, ent, stats, tl, ti};
+}
+
+// d logits, contiguous in the logits' shape and dtype
+at::Tensor token_logprobs_bwd(const at::Tensor& z, const at::Tensor& target, const at::Tensor& stats, int64_t ignore_index,
+                              double inv_t, const c10::optional<at::Tensor>& dlogp, const c10::optional<at::Tensor>& dent) {
+  const LogitRows r = logit_rows(z, target, "token_logprobs_bwd");
+  for (const auto* t : {&dlogp, &dent})
+    if (t->has_value() && (*t)->defined())
+      TORCH_CHECK((*t)->scalar_type() == at::kFloat && (*t)->is_contiguous() && (*t)->numel() == r.rows &&
+                      (*t)->device() == z.device(),
+                  "token_logprobs_bwd: contiguous fp32 gradients, one for each row");
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 3 * r.rows &&
+                  stats.device() == z.device(), "token_logprobs_bwd: the forward's stats [rows, 3]");
+  const at::DeviceGuard guard(z.device());
+  auto dz = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous));
+  HYP_CHECK_HIP(hyp::token_logprobs_bwd(dtype_code(z), z.data_ptr(), r.s0, r.s1, r.inner, r.rows, r.V,
+                                        target.data_ptr<int64_t>(), ignore_index, (float)inv_t, stats.data_ptr<float>(),
+                                        ptr_or_null<float>(dlogp), ptr_or_null<float>(dent), dz.data_ptr(), cur_stream()));
+  return dz;
+}
+
 // ---- classifier head + MSE (linear_mse.hip) -----------------------------------------------------
 void check_head(const at::Tensor& x, const at::Tensor& w, const char* who) {
   HYP_CHECK_CUDA_TENSOR(x);
@@ -122,6 +184,12 @@ at::Tensor embedding_bwd(const at::Tensor& dy, const at::Tensor& ids, int64_t V,
 
 void register_loss_ops(pybind11::module& m) {
   m.def("embedding_fwd", &embedding_fwd, "token embedding gather");
+  m.def("token_logprobs_fwd", &token_logprobs_fwd, "log probability of each row's target, entropy, top-k alternatives",
+        pybind11::arg("logits"), pybind11::arg("target"), pybind11::arg("k"), pybind11::arg("ignore_index"),
+        pybind11::arg("inv_t"));
+  m.def("token_logprobs_bwd", &token_logprobs_bwd, "gradient of token_logprobs_fwd's log probabilities and entropies",
+        pybind11::arg("logits"), pybind11::arg("target"), pybind11::arg("stats"), pybind11::arg("ignore_index"),
+        pybind11::arg("inv_t"), pybind11::arg("dlogp"), pybind11::arg("dent"));
   m.def("linear_mse_fwd", &linear_mse_fwd, "classifier head + MSE forward (loss, fp32 dz)", pybind11::arg("x"),
         pybind11::arg("w"), pybind11::arg("b"), pybind11::arg("y"));
   m.def("linear_mse_bwd", &linear_mse_bwd, "classifier head + MSE backward (dx, dw, db) in one launch",

@@ -129,6 +129,21 @@ hipError_t cross_entropy_fwd_bwd(int dtype, void* logits, int64_t rows, int V, i
 }  // namespace hyp
 
 namespace hyp {
+// ---- token_logprobs.hip ------------------------------------------------------------------------
+// Rows of V logits with unit element stride: row r at (r / inner) * s0 + (r % inner) * s1 elements.
+// stats [rows, 3] is what the backward needs; top_* [rows, k].  dlogp / dent may be null (zeros); dz is
+// contiguous [rows, V].  A launch holds fewer than kTokenRowsMax workgroups of 256 threads.
+constexpr int kTokenTopMax = 32;
+constexpr int64_t kTokenRowsMax = int64_t(1) << 24;
+hipError_t token_logprobs_fwd(int dtype, const void* z, int64_t s0, int64_t s1, int inner, int64_t rows, int V,
+                              const int64_t* target, int64_t ignore, float inv_t, float* logp, float* ent, float* stats,
+                              int k, float* top_lp, int64_t* top_id, hipStream_t stream);
+hipError_t token_logprobs_bwd(int dtype, const void* z, int64_t s0, int64_t s1, int inner, int64_t rows, int V,
+                              const int64_t* target, int64_t ignore, float inv_t, const float* stats,
+                              const float* dlogp, const float* dent, void* dz, hipStream_t stream);
+}  // namespace hyp
+
+namespace hyp {
 // ---- rope_swiglu.hip -------------------------------------------------------------------------
 // q [tokens, Hq, D], k [tokens, Hk, D] with token / head strides in elements (unit stride in D);
 // pos: int64 [tokens] or null (position = token % S).  inverse=1 rotates by -angle (backward).

@@ -1,0 +1,414 @@
+// Log probabilities of given tokens, the entropy of each row and its most likely tokens, and the
+// gradient of the first two into the logits.
+//
+// Per row of logits z with y = z / T, in base 2 (c = log2(e) / T, t_j = (z_j - m) c, m the row's
+// largest logit; the difference first, so that a row of the type's lowest value stays finite), one
+// pass with a running maximum:
+//   s = sum 2^t_j,  u = sum 2^t_j t_j
+//   logprob = (z_target - m) / T - log2 s ln 2,   H = (log2 s - u / s) ln 2
+// and from the saved (m, log2 s, H), with q_j = t_j - log2 s, p_j = 2^q_j:
+//   dz_j = [ dlogp (delta_j - p_j) - dH p_j (q_j ln 2 + H) ] / T
+// Sums are fp32.  The forward reads every logit once, the backward reads it once and writes its
+// gradient once: HBM bounds both (about 10 VALU slots per logit, of which exp2 takes 4).
+//
+// Rows start at any element (V = 50257 rows of 2-byte logits are 2-byte aligned): 16-byte loads and
+// stores at the row's own alignment, which gfx950 global memory takes, instead of a scalar head.
+//
+// An empty row (every logit -inf) has logprob -inf, entropy 0 and no gradient; a NaN or +inf logit
+// makes its row's results and gradient NaN; a target outside [0, V) is never read and makes the
+// row's logprob and gradient NaN; a row whose target is ignore_index is not read: 0 everywhere, ids -1.
+#include "hyp_common.h"
+#include "hyp_kernels.h"
+
+namespace hyp {
+namespace {
+
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kFloor = -200.f;  // 2^-200 is 0 in fp32: a finite stand-in for -inf in products with p = 0
+constexpr int kTopCap = 1024;     // candidates of the top alternatives kept in LDS
+
+typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename T>
+struct Row16 {  // 16 bytes of a row, at the row's alignment
+  static constexpr int N = 16 / (int)sizeof(T);
+  static __device__ __forceinline__ u32x4a raw(const T* p) { return *reinterpret_cast<const u32x4a*>(p); }
+  static __device__ __forceinline__ void open(const u32x4a& r, float (&v)[N]);
+};
+template <>
+__device__ __forceinline__ void Row16<float>::open(const u32x4a& r, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <>
+__device__ __forceinline__ void Row16<bf16_t>::open(const u32x4a& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(r[i] << 16);
+    v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void Row16<f16_t>::open(const u32x4a& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = f16_lo(r[i]);
+    v[2 * i + 1] = f16_hi(r[i]);
+  }
+}
+
+__device__ __forceinline__ u32x4a close16(const float (&v)[4], const float*) {
+  return u32x4a{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+}
+__device__ __forceinline__ u32x4a close16(const float (&v)[8], const bf16_t*) {
+  return u32x4a{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+}
+__device__ __forceinline__ u32x4a close16(const float (&v)[8], const f16_t*) {
+  return u32x4a{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7])};
+}
+
+// running (m, s, u) of a set of logits: m the largest logit, s = sum 2^((z - m) c), u = sum of the
+// same weighted by its exponent.  NaN stays in s; m = -inf with s = 0 is the empty set.
+struct Run {
+  float m, s, u;
+};
+
+__device__ __forceinline__ Run run_join(const Run& a, const Run& b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  const float da = a.m == m ? 0.f : (a.m - m) * c, db = b.m == m ? 0.f : (b.m - m) * c;
+  const float fa = exp2f(da), fb = exp2f(db);
+  return {m, a.s * fa + b.s * fb, fa * (a.u + fmaxf(da, kFloor) * a.s) + fb * (b.u + fmaxf(db, kFloor) * b.s)};
+}
+
+template <int N>
+__device__ __forceinline__ void run_add(Run& r, const float (&v)[N], float c) {
+  float m = r.m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
+  if (m > r.m) {  // also the first values: from m = -inf the old sums are 0
+    const float d = (r.m - m) * c, f = exp2f(d);
+    r.u = f * (r.u + fmaxf(d, kFloor) * r.s);
+    r.s *= f;
+    r.m = m;
+  }
+  const float at = r.m == -INFINITY ? 0.f : r.m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float t = (v[i] - at) * c, e = __builtin_amdgcn_exp2f(t);
+    r.s += e;
+    r.u = fmaf(e, fmaxf(t, kFloor), r.u);
+  }
+}
+
+// order of the alternatives: larger logit first (NaN above everything, -0 = +0), then the lower id
+__device__ __forceinline__ uint64_t top_key(float z, int id) {
+  const uint32_t b = __float_as_uint(z + 0.f);
+  uint32_t k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  if (z != z) k = 0xffffffffu;
+  return ((uint64_t)k << 32) | (0xffffffffu - (uint32_t)id);
+}
+__device__ __forceinline__ uint64_t shfl_max64(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t w = __shfl_xor((unsigned long long)v, o, 64);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+struct LpArgs {
+  const void* z;
+  int64_t s0, s1;  // element strides of row r: (r / inner) * s0 + (r % inner) * s1
+  int inner, V;
+  const int64_t* target;
+  int64_t ignore;
+  float c, inv_t;
+  float *logp, *ent, *stats;  // stats [rows, 3]: m, log2 s, H
+  int k;
+  float* top_lp;
+  int64_t* top_id;
+};
+
+template <typename T>
+__device__ __forceinline__ const T* row_ptr(const LpArgs& a, int64_t r) {
+  return static_cast<const T*>(a.z) + (r / a.inner) * a.s0 + (r % a.inner) * a.s1;
+}
+
+// One workgroup per row.  TOP: also the k most likely tokens.
+//   1. every thread keeps the key of its largest logit during the pass; the r-th largest of each
+//      full wave, r = ceil(k / full waves), bounds the k-th largest of the row from below (their
+//      smallest is passed by at least k logits);
+//   2. a second sweep (cache) collects the keys that reach the bound into LDS, about 2k..6k of them,
+//      and every candidate writes itself to the place given by how many are larger.
+//   Were there more candidates than fit (orders made to do so), k sweeps pick one maximum each.
+template <typename T, int THREADS, bool TOP>
+__global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
+  constexpr int N = Row16<T>::N, W = THREADS / 64, U = 4;
+  __shared__ Run wr[W];
+  __shared__ uint64_t cand[TOP ? kTopCap : 1];
+  __shared__ uint64_t wkey[W];
+  __shared__ int ncand;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t tgt = a.target[row];
+  if (tgt == a.ignore) {
+    if (tid == 0) {
+      a.logp[row] = 0.f;
+      a.ent[row] = 0.f;
+      a.stats[3 * row] = a.stats[3 * row + 1] = a.stats[3 * row + 2] = 0.f;
+    }
+    if (TOP && tid < a.k) {
+      a.top_lp[row * a.k + tid] = 0.f;
+      a.top_id[row * a.k + tid] = -1;
+    }
+    return;
+  }
+  const T* z = row_ptr<T>(a, row);
+  const int nv = a.V / N, tail = nv * N;
+  Run run{-INFINITY, 0.f, 0.f};
+  uint64_t best = 0;
+  auto take = [&](const u32x4a& raw, int v) {
+    float x[N];
+    Row16<T>::open(raw, x);
+    run_add<N>(run, x, a.c);
+    if (TOP) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint64_t k = top_key(x[i], v * N + i);
+        best = k > best ? k : best;
+      }
+    }
+  };
+  int v = tid;
+  for (; v + (U - 1) * THREADS < nv; v += U * THREADS) {
+    u32x4a r[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) r[i] = Row16<T>::raw(z + (int64_t)(v + i * THREADS) * N);
+#pragma unroll
+    for (int i = 0; i < U; ++i) take(r[i], v + i * THREADS);
+  }
+  for (; v < nv; v += THREADS) take(Row16<T>::raw(z + (int64_t)v * N), v);
+  if (tail + tid < a.V) {
+    const float x[1] = {ld1<T>(z + tail + tid)};
+    run_add<1>(run, x, a.c);
+    if (TOP) {
+      const uint64_t k = top_key(x[0], tail + tid);
+      best = k > best ? k : best;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    run = run_join(run, Run{__shfl_xor(run.m, o, 64), __shfl_xor(run.s, o, 64), __shfl_xor(run.u, o, 64)}, a.c);
+  if (lane == 0) wr[wv] = run;
+  int full = 0;
+  if (TOP) {
+    full = min(W, nv / 64);  // waves whose every thread holds a logit
+    if (wv < full) {
+      const int rounds = (a.k + full - 1) / full;
+      uint64_t mine = best, top = 0;
+      for (int i = 0; i < rounds; ++i) {
+        top = shfl_max64(mine);
+        if (mine == top) mine = 0;  // keys differ in their ids
+      }
+      if (lane == 0) wkey[wv] = top;
+    }
+    if (tid == 0) ncand = 0;
+  }
+  __syncthreads();
+  run = lane < W ? wr[lane] : Run{-INFINITY, 0.f, 0.f};
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1)
+    run = run_join(run, Run{__shfl_xor(run.m, o, 64), __shfl_xor(run.s, o, 64), __shfl_xor(run.u, o, 64)}, a.c);
+  run = {__shfl(run.m, 0, 64), __shfl(run.s, 0, 64), __shfl(run.u, 0, 64)};
+  const bool empty = run.s == 0.f;  // NaN is not
+  const float m = empty ? 0.f : run.m, ls = empty ? INFINITY : __log2f(run.s);
+  if (tid == 0) {
+    float lp = __uint_as_float(0x7fc00000u);
+    if (tgt >= 0 && tgt < a.V) lp = empty ? -INFINITY : fmaf(ld1<T>(z + tgt) - m, a.inv_t, -ls * kLn2);
+    float h = empty ? 0.f : (ls - run.u / run.s) * kLn2;
+    if (h < 0.f) h = 0.f;  // rounding, in a row of one token
+    a.logp[row] = lp;
+    a.ent[row] = h;
+    a.stats[3 * row] = m;
+    a.stats[3 * row + 1] = ls;
+    a.stats[3 * row + 2] = h;
+  }
+  if (!TOP) return;
+  uint64_t bound = full > 0 ? wkey[0] : 0;
+  for (int i = 1; i < full; ++i) bound = wkey[i] < bound ? wkey[i] : bound;
+  auto put = [&](float x, int id) {
+    const uint64_t k = top_key(x, id);
+    if (k >= bound) {
+      const int at = atomicAdd(&ncand, 1);
+      if (at < kTopCap) cand[at] = k;
+    }
+  };
+  for (v = tid; v < nv; v += THREADS) {
+    float x[N];
+    Row16<T>::open(Row16<T>::raw(z + (int64_t)v * N), x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(x[i], v * N + i);
+  }
+  if (tail + tid < a.V) put(ld1<T>(z + tail + tid), tail + tid);
+  __syncthreads();
+  const int n = ncand;
+  auto write = [&](int at, uint64_t key) {
+    const int id = (int)(0xffffffffu - (uint32_t)key);
+    a.top_id[row * a.k + at] = id;
+    a.top_lp[row * a.k + at] = empty ? -INFINITY : fmaf(ld1<T>(z + id) - m, a.inv_t, -ls * kLn2);
+  };
+  if (n <= kTopCap) {
+    for (int i = tid; i < n; i += THREADS) {
+      const uint64_t key = cand[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += cand[j] > key;
+      if (rank < a.k) write(rank, key);
+    }
+    return;
+  }
+  uint64_t last = ~0ull;
+  for (int i = 0; i < a.k; ++i) {
+    best = 0;
+    auto look = [&](float x, int id) {
+      const uint64_t k = top_key(x, id);
+      if (k < last && k > best) best = k;
+    };
+    for (v = tid; v < nv; v += THREADS) {
+      float x[N];
+      Row16<T>::open(Row16<T>::raw(z + (int64_t)v * N), x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) look(x[j], v * N + j);
+    }
+    if (tail + tid < a.V) look(ld1<T>(z + tail + tid), tail + tid);
+    best = shfl_max64(best);
+    __syncthreads();
+    if (lane == 0) wkey[wv] = best;
+    __syncthreads();
+    last = wkey[0];
+    for (int j = 1; j < W; ++j) last = wkey[j] > last ? wkey[j] : last;
+    if (tid == 0) write(i, last);
+  }
+}
+
+constexpr int kBwdThreads = 256, kBwdU = 4;
+
+// grid (chunks, rows): a workgroup writes kBwdThreads * kBwdU 16-byte pieces of one row's gradient
+template <typename T>
+__global__ __launch_bounds__(kBwdThreads) void token_lp_bwd_k(const LpArgs a, const float* __restrict__ dlogp,
+                                                              const float* __restrict__ dent, T* __restrict__ dz,
+                                                              int chunks) {
+  constexpr int N = Row16<T>::N;
+  const int64_t row = blockIdx.x / chunks;
+  const int chunk = blockIdx.x % chunks;
+  const int64_t tgt = a.target[row];
+  const bool ignored = tgt == a.ignore;
+  T* g = dz + row * a.V;
+  const int nv = a.V / N, tail = nv * N;
+  const int v0 = chunk * (kBwdThreads * kBwdU) + threadIdx.x;
+  const float m = a.stats[3 * row], ls = a.stats[3 * row + 1], h = a.stats[3 * row + 2];
+  float wl = 0.f, wh = 0.f;  // both 0 in an ignored or empty row
+  if (!ignored && ls != INFINITY) {
+    wl = dlogp ? dlogp[row] : 0.f;
+    wh = dent ? dent[row] : 0.f;
+    if (tgt < 0 || tgt >= a.V) wl = __uint_as_float(0x7fc00000u);
+  }
+  const float hot = wl * a.inv_t;
+  // dz = -p (A + B q),  A = (wl + wh H) / T,  B = wh ln2 / T
+  const float A = (wl + wh * h) * a.inv_t, B = wh * kLn2 * a.inv_t;
+  auto grad = [&](float x, int id) {
+    const float q = (x - m) * a.c - ls;
+    const float d = -__builtin_amdgcn_exp2f(q) * fmaf(B, fmaxf(q, kFloor), A);
+    return id == tgt ? d + hot : d;
+  };
+  if (ignored) {
+    const u32x4a zero{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kBwdU; ++i) {
+      const int v = v0 + i * kBwdThreads;
+      if (v < nv) *reinterpret_cast<u32x4a*>(g + (int64_t)v * N) = zero;
+    }
+    if (chunk == 0 && tail + (int)threadIdx.x < a.V) st1<T>(g + tail + threadIdx.x, 0.f);
+    return;
+  }
+  const T* z = row_ptr<T>(a, row);
+  u32x4a r[kBwdU];
+#pragma unroll
+  for (int i = 0; i < kBwdU; ++i) {
+    const int v = v0 + i * kBwdThreads;
+    if (v < nv) r[i] = Row16<T>::raw(z + (int64_t)v * N);
+  }
+#pragma unroll
+  for (int i = 0; i < kBwdU; ++i) {
+    const int v = v0 + i * kBwdThreads;
+    if (v < nv) {
+      float x[N];
+      Row16<T>::open(r[i], x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = grad(x[j], v * N + j);
+      *reinterpret_cast<u32x4a*>(g + (int64_t)v * N) = close16(x, (const T*)nullptr);
+    }
+  }
+  if (chunk == 0 && tail + (int)threadIdx.x < a.V)
+    st1<T>(g + tail + threadIdx.x, grad(ld1<T>(z + tail + threadIdx.x), tail + threadIdx.x));
+}
+
+LpArgs lp_args(const void* z, int64_t s0, int64_t s1, int inner, int V, const int64_t* target, int64_t ignore,
+               float inv_t) {
+  LpArgs a{};
+  a.z = z;
+  a.s0 = s0;
+  a.s1 = s1;
+  a.inner = inner;
+  a.V = V;
+  a.target = target;
+  a.ignore = ignore;
+  a.inv_t = inv_t;
+  a.c = inv_t * 1.4426950408889634f;
+  return a;
+}
+
+}  // namespace
+
+hipError_t token_logprobs_fwd(int dtype, const void* z, int64_t s0, int64_t s1, int inner, int64_t rows, int V,
+                              const int64_t* target, int64_t ignore, float inv_t, float* logp, float* ent, float* stats,
+                              int k, float* top_lp, int64_t* top_id, hipStream_t stream) {
+  if (rows == 0) return hipSuccess;
+  if (V < 1 || inner < 1 || k < 0 || k > kTokenTopMax || k > V || rows >= kTokenRowsMax) return hipErrorInvalidValue;
+  LpArgs a = lp_args(z, s0, s1, inner, V, target, ignore, inv_t);
+  a.logp = logp;
+  a.ent = ent;
+  a.stats = stats;
+  a.k = k;
+  a.top_lp = top_lp;
+  a.top_id = top_id;
+  const bool wide = rows < 512 && V > 8192;
+  HYP_DISPATCH_FLOAT(dtype, T, {
+    if (k > 0) {
+      if (wide) hipLaunchKernelGGL((token_lp_fwd_k<T, 1024, true>), dim3(rows), dim3(1024), 0, stream, a);
+      else hipLaunchKernelGGL((token_lp_fwd_k<T, 256, true>), dim3(rows), dim3(256), 0, stream, a);
+    } else {
+      if (wide) hipLaunchKernelGGL((token_lp_fwd_k<T, 1024, false>), dim3(rows), dim3(1024), 0, stream, a);
+      else hipLaunchKernelGGL((token_lp_fwd_k<T, 256, false>), dim3(rows), dim3(256), 0, stream, a);
+    }
+  });
+  return hipGetLastError();
+}
+
+hipError_t token_logprobs_bwd(int dtype, const void* z, int64_t s0, int64_t s1, int inner, int64_t rows, int V,
+                              const int64_t* target, int64_t ignore, float inv_t, const float* stats,
+                              const float* dlogp, const float* dent, void* dz, hipStream_t stream) {
+  if (rows == 0) return hipSuccess;
+  if (V < 1 || inner < 1) return hipErrorInvalidValue;
+  LpArgs a = lp_args(z, s0, s1, inner, V, target, ignore, inv_t);
+  a.stats = const_cast<float*>(stats);
+  HYP_DISPATCH_FLOAT(dtype, T, {
+    const int per = kBwdThreads * kBwdU * Row16<T>::N;
+    const int64_t chunks = (V + per - 1) / per;
+    if (rows * chunks >= kTokenRowsMax) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((token_lp_bwd_k<T>), dim3(rows * chunks), dim3(kBwdThreads), 0, stream, a, dlogp, dent,
+                       static_cast<T*>(dz), (int)chunks);
+  });
+  return hipGetLastError();
+}
+
+}  // namespace hyp

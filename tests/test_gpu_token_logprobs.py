@@ -1,0 +1,152 @@
+"""token_logprobs kernels against the 64-bit oracle: types, odd sizes, strides, masks, ties, graphs, streams."""
+import math
+
+import pytest
+import torch
+
+from hyperion.ops import _native
+from hyperion.ops.token_logprobs import token_logprobs
+
+from token_logprobs_oracle import bounds, check, oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def rows(R, V, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    z = (torch.randn(R, V, generator=g) * 2.5).to(dtype)
+    return z, torch.randint(V, (R,), generator=g), torch.randn(R, generator=g), torch.randn(R, generator=g)
+
+
+def compare(z, t, dlogp, dent, k, temperature=1.0, ref=None):
+    """`ref`: the oracle's rows where z is a view of another shape."""
+    ref = z if ref is None else ref
+    zd = z.detach().requires_grad_(True)
+    n = _native.counters().get("token_logprobs", 0)
+    out = token_logprobs(zd, t.to(DEV).view(z.shape[:-1]), top_k=k, temperature=temperature)
+    assert _native.counters()["token_logprobs"] == n + 1
+    g, = torch.autograd.grad([out.logprobs, out.entropy], [zd], [dlogp.to(DEV).view(z.shape[:-1]), dent.to(DEV).view(z.shape[:-1])])
+    V = z.shape[-1]
+    want = oracle(ref, t, k, -100, temperature, dlogp, dent)
+    b = bounds(ref, temperature, dlogp, dent, want)
+    check(out.logprobs.view(-1), want[0], b[0])
+    check(out.entropy.view(-1), want[1], b[1])
+    if k:
+        assert torch.equal(out.top_ids.view(-1, k).cpu(), want[3])
+        check(out.top_logprobs.view(-1, k), want[2], b[2])
+    check(g.view(-1, V), want[4], b[3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,V,k", [(1, 1, 1), (3, 2, 2), (2, 7, 0), (5, 33, 32), (3, 509, 5), (4, 1000, 32), (2, 2049, 20),
+                                   (3, 8193, 1), (2, 50257, 20), (1, 130001, 32), (530, 1003, 3), (520, 4, 0)])
+def test_against_oracle(R, V, k, dtype):
+    z, t, a, b = rows(R, V, dtype, R + V)
+    if R > 2:
+        t[1] = -100
+    compare(z.to(DEV), t, a, b, k, temperature=1.0 if V % 2 else 0.7)
+
+
+@pytest.mark.parametrize("V", [65, 9001])
+def test_masked_empty_and_poisoned_rows(V):
+    z, t, a, b = rows(9, V, torch.bfloat16)
+    z[0] = -math.inf
+    z[1, 3:] = -math.inf  # fewer tokens left than alternatives asked for
+    t[1] = 40
+    z[2, 7] = math.nan
+    z[3, 9] = math.inf
+    t[4] = V
+    t[5] = -7
+    z[6] = -math.inf
+    z[6, 11] = 2.0
+    t[6] = 11
+    z[7] = torch.finfo(torch.bfloat16).min  # a mask of the type's lowest value everywhere
+    z[8, ::2] = torch.finfo(torch.bfloat16).min
+    compare(z.to(DEV), t, a, b, 8)
+
+
+@pytest.mark.parametrize("R", [2, 515])
+def test_ties_go_to_the_lowest_id(R):
+    V = 9000
+    z = torch.zeros(R, V, dtype=torch.bfloat16)
+    z[0, 1::2] = -0.0
+    z[1] = torch.arange(V) // 3 % 7
+    t, a = torch.zeros(R, dtype=torch.long), torch.ones(R)
+    compare(z.to(DEV), t, a, a, 32)
+
+
+def test_more_candidates_than_fit():
+    # the first thread of every wave holds all of the row's largest logits: the bound passes thousands
+    V = 130000
+    z = torch.zeros(1, V)
+    v = torch.arange(V) // 4
+    z[0] = torch.where(v % 64 < 2, torch.arange(V) % 997 * 1e-3 + 1, -torch.arange(V) * 1e-6)
+    compare(z.to(DEV), torch.tensor([5]), torch.ones(1), torch.ones(1), 32)
+
+
+def test_strided_views_are_read_in_place():
+    B, S, V = 3, 5, 501
+    g = torch.Generator().manual_seed(1)
+    full = (torch.randn(B, S, V + 3, generator=g) * 2).bfloat16().to(DEV)
+    view = full[:, :-1, 1:V + 1]  # rows at odd elements, a gap after every batch entry
+    t = torch.randint(V, (B * (S - 1),), generator=g)
+    a, b = torch.randn(t.numel(), generator=g), torch.randn(t.numel(), generator=g)
+    compare(view, t, a, b, 5, ref=view.reshape(-1, V))
+    keep = full.clone()
+    token_logprobs(view, t.to(DEV).view(B, S - 1))
+    assert torch.equal(full, keep)
+    swapped = full.transpose(0, 1)[..., :V]
+    t2 = torch.randint(V, (S * B,), generator=g)
+    a2 = torch.randn(S * B, generator=g)
+    compare(swapped, t2, a2, a2, 3, ref=swapped.reshape(-1, V))
+    column = full.permute(0, 2, 1)[:, :S, :]  # no unit stride in the last dimension: copied
+    t3 = torch.randint(S, (B * S,), generator=g)
+    compare(column, t3, a2[:B * S], a2[:B * S], 2, ref=column.reshape(-1, S))
+
+
+def test_one_gradient_alone_and_none():
+    z, t, a, _ = rows(4, 777, torch.float32)
+    zd = z.to(DEV).requires_grad_(True)
+    for pick in ("logprobs", "entropy"):
+        o = token_logprobs(zd, t.to(DEV))
+        g, = torch.autograd.grad(getattr(o, pick).sum(), zd)
+        one, zero = torch.ones(4), torch.zeros(4)
+        w = (one, zero) if pick == "logprobs" else (zero, one)
+        want = oracle(z, t, 0, -100, 1.0, *w)
+        check(g, want[4], bounds(z, 1.0, *w, want)[3])
+    with torch.no_grad():
+        assert not token_logprobs(zd, t.to(DEV)).logprobs.requires_grad
+    empty = token_logprobs(zd[:0], t.to(DEV)[:0], top_k=2)
+    assert empty.logprobs.shape == (0,) and torch.autograd.grad(empty.logprobs.sum(), zd)[0].abs().sum() == 0
+
+
+def test_other_stream_and_graph_replays():
+    z, t, a, b = rows(6, 50257, torch.bfloat16)
+    zd, td, ad, bd = (x.to(DEV) for x in (z, t, a, b))
+
+    def step(x):
+        x = x.detach().requires_grad_(True)
+        o = token_logprobs(x, td, top_k=5)
+        return [o.logprobs.detach(), o.entropy.detach(), o.top_logprobs, o.top_ids,
+                torch.autograd.grad([o.logprobs, o.entropy], [x], [ad, bd])[0]]
+
+    want = step(zd)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step(zd)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    static = zd.clone()
+    with torch.cuda.stream(s):
+        step(static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for i in range(3):
+        static.copy_(torch.roll(zd, i, 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, step(static)))
