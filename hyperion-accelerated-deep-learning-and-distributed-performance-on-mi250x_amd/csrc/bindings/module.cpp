@@ -26,6 +26,7 @@ PYBIND11_MODULE(HYP_MODULE_NAME, m) {
   hypbind::register_conv_ops(m);
   hypbind::register_rng_ops(m);
   hypbind::register_ws_ops(m);
+  hypbind::register_mx_ops(m);
   // segmented hipGraph capture (train/segments.py): has the capture on `stream` recorded any work
   // yet?  An open capture with no leaf node is still empty — a hole right after it merges into the
   // previous hole instead of leaving an empty graph segment to end and replay

@@ -12,4 +12,5 @@ void register_comm(pybind11::module& m);
 void register_conv_ops(pybind11::module& m);
 void register_rng_ops(pybind11::module& m);
 void register_ws_ops(pybind11::module& m);
+void register_mx_ops(pybind11::module& m);
 }  // namespace hypbind

@@ -144,6 +144,25 @@ hipError_t token_logprobs_bwd(int dtype, const void* z, int64_t s0, int64_t s1, 
 }  // namespace hyp
 
 namespace hyp {
+// ---- mxfp4.hip ---------------------------------------------------------------------------------
+// Microscaled 4-bit rows: codes [rows, 16 nb] bytes, scales [rows, nb] bytes, nb = ceil(cols / 32).
+constexpr int64_t kMxGridMax = int64_t(1) << 24;  // workgroups of a launch
+hipError_t mx_quantize(int dtype, const void* x, int64_t ld, int64_t rows, int cols, uint8_t* codes, uint8_t* scales,
+                       hipStream_t stream);
+hipError_t mx_dequantize(int dtype, const uint8_t* codes, const uint8_t* scales, int64_t rows, int cols, void* out,
+                         int64_t pitch, hipStream_t stream);
+// x [rows, cols] -> bf16 pieces [P, rows, pitch] whose sum is x exactly (P = 1 bf16, 2 fp16, 3 fp32)
+hipError_t mx_pieces(int dtype, const void* x, int64_t ld, int64_t rows, int cols, int pitch, void* out,
+                     hipStream_t stream);
+// y [rows, cols] = sum of the fp32 slabs part [pieces, rows, pitch] (+ bias)
+hipError_t mx_join(int dtype, const float* part, int pieces, int64_t rows, int cols, int64_t pitch, const float* bias,
+                   void* y, hipStream_t stream);
+// y [M, N] (bf16 / fp32) = x [M, 32 nb] (bf16) times the transpose of the 4-bit weight [N, 32 nb] (+ bias)
+hipError_t mx_rows(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
+                   int out_dtype, void* y, hipStream_t stream);
+}  // namespace hyp
+
+namespace hyp {
 // ---- rope_swiglu.hip -------------------------------------------------------------------------
 // q [tokens, Hq, D], k [tokens, Hk, D] with token / head strides in elements (unit stride in D);
 // pos: int64 [tokens] or null (position = token % S).  inverse=1 rotates by -angle (backward).

@@ -1,0 +1,155 @@
+"""MXFP4 kernels against the 64-bit oracle: types, odd sizes, strides, edges, both products, graphs, streams."""
+import math
+
+import pytest
+import torch
+
+from hyperion.ops import _native
+from hyperion.ops.mxfp4 import MXFP4Tensor, mxfp4_linear, quantize_mxfp4
+
+from mxfp4_oracle import decoded, product_bound, quantized_values
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def same(got, want):
+    got = got.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,K", [(1, 1), (3, 31), (2, 64), (5, 100), (1023, 500), (70, 4096)])
+def test_quantize_against_oracle(R, K, dtype):
+    x = torch.randn(R, K, generator=torch.Generator().manual_seed(K)).to(dtype)
+    q = quantize_mxfp4(x.to(DEV))
+    want = quantized_values(x)
+    same(q.dequantize(torch.float32), want)
+    same(q.dequantize(torch.bfloat16), want)
+    same(q.dequantize(torch.float16), want.half().double())
+    assert torch.equal(decoded(q.codes, q.scales, K), want)
+    ref = quantize_mxfp4(x)
+    assert torch.equal(q.codes.cpu(), ref.codes) and torch.equal(q.scales.cpu(), ref.scales)
+
+
+def test_quantize_edges_and_strides():
+    x = torch.zeros(7, 64)
+    x[0, :16] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, 4.0])
+    x[1, 3], x[1, 40] = math.nan, 1.0
+    x[2, 3], x[2, 40] = -math.inf, 1.0
+    x[3] = torch.linspace(0, 3e38, 64)
+    x[4] = torch.linspace(0, 3e-38, 64)
+    x[5, 0] = -0.0
+    x[6] = torch.linspace(0, 3e-44, 64)
+    same(quantize_mxfp4(x.to(DEV)).dequantize(torch.float32), quantized_values(x))
+    y = torch.randn(9, 77, generator=torch.Generator().manual_seed(1)).bfloat16()
+    yd = y.to(DEV)
+    same(quantize_mxfp4(yd[:, 3:70]).dequantize(torch.float32), quantized_values(y[:, 3:70]))  # rows at odd elements
+    same(quantize_mxfp4(yd.t()).dequantize(torch.float32), quantized_values(y.t()))
+    same(quantize_mxfp4(yd[None, ::2]).dequantize(torch.float32)[0], quantized_values(y[::2]))
+    assert quantize_mxfp4(yd[:0]).dequantize().shape == (0, 77)
+
+
+def check_linear(M, N, K, dtype, bias, seed=0, view=lambda t: t):
+    g = torch.Generator().manual_seed(seed + M + N + K)
+    w = quantize_mxfp4(torch.randn(N, K, generator=g).to(DEV))
+    x = view(torch.randn(M, K, generator=g).to(dtype).to(DEV)).detach().requires_grad_(True)
+    b = torch.randn(N, generator=g).to(DEV).requires_grad_(True) if bias else None
+    dy = torch.randn(x.shape[0], N, generator=g).to(dtype).to(DEV)
+    y = mxfp4_linear(x, w, b)
+    dx = torch.autograd.grad(y, x, dy)[0]
+    # the oracle's products run on the device in fp64
+    W = decoded(w.codes, w.scales, K).to(DEV)
+    xd, dd = x.detach().double(), dy.double()
+    want, bound = xd @ W.t(), product_bound(xd, W.t(), dtype)
+    if bias:
+        want = want + b.detach().double()
+        bound = bound + (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * (b.detach().double().abs() + want.abs())
+    assert y.dtype == dtype and ((y.detach().double() - want).abs() <= bound).all()
+    assert dx.dtype == dtype and ((dx.double() - dd @ W).abs() <= product_bound(dd, W, dtype)).all()
+    return w, x, dy, y, dx
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 16, 32), (1, 1, 1), (3, 7, 33), (16, 100, 1000), (17, 200, 129), (40, 24, 64),
+                                   (64, 50, 4096), (65, 100, 100), (130, 257, 500), (300, 1000, 768), (1, 4096, 4096)])
+def test_linear_against_oracle(M, N, K, dtype):
+    check_linear(M, N, K, dtype, bias=M % 2 == 1)
+
+
+@pytest.mark.parametrize("M", [1, 5, 96])
+def test_strided_activations(M):
+    check_linear(M, 40, 96, torch.bfloat16, True, view=lambda t: torch.cat([t, t], 1)[:, 1:97])
+    check_linear(96, 40, M, torch.bfloat16, False, view=lambda t: t.t().contiguous().t())
+
+
+def test_both_sides_of_the_row_limit_agree_in_dtype_and_shape():
+    for M in (64, 65):
+        w, x, dy, y, dx = check_linear(M, 64, 96, torch.bfloat16, False)
+        y3 = mxfp4_linear(x.view(1, M, 96), w)
+        assert torch.equal(y3[0], y)  # deterministic, and batch dimensions are rows
+
+
+def test_non_finite_activations_and_weights():
+    g = torch.Generator().manual_seed(5)
+    wv = torch.randn(32, 64, generator=g)
+    wv[3, 40] = math.nan
+    w = quantize_mxfp4(wv.to(DEV))
+    for dtype in DTYPES:
+        for M in (2, 70):
+            x = torch.randn(M, 64, generator=g).to(dtype)
+            x[1, 5] = math.inf
+            y = mxfp4_linear(x.to(DEV), w).cpu()
+            want = x.double() @ decoded(w.codes, w.scales, 64).t()
+            assert torch.equal(torch.isfinite(y), torch.isfinite(want))
+            assert torch.isnan(y[0, 3]) and torch.isfinite(y[0, 4])
+
+
+def test_misaligned_codes_are_taken():
+    q = quantize_mxfp4(torch.randn(8, 64, device=DEV))
+    buf = torch.empty(q.codes.numel() + 1, dtype=torch.uint8, device=DEV)
+    buf[1:] = q.codes.view(-1)
+    m = MXFP4Tensor(buf[1:].view(8, 32), q.scales, q.shape)
+    x = torch.randn(3, 64, device=DEV, dtype=torch.bfloat16)
+    assert torch.equal(mxfp4_linear(x, m), mxfp4_linear(x, q))
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_other_stream_and_graph_replays(M):
+    w = quantize_mxfp4(torch.randn(320, 512, device=DEV) * 0.05)
+    x = torch.randn(M, 512, device=DEV, dtype=torch.bfloat16)
+    dy = torch.randn(M, 320, device=DEV, dtype=torch.bfloat16)
+
+    def step(t):
+        t = t.detach().requires_grad_(True)
+        y = mxfp4_linear(t, w)
+        return [y.detach(), torch.autograd.grad(y, t, dy)[0], quantize_mxfp4(t).codes]
+
+    want = step(x)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step(x)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    static = x.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for i in range(3):
+        static.copy_(torch.roll(x, i, 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step(static)))
+
+
+def test_kernels_are_reached():
+    w = quantize_mxfp4(torch.randn(64, 64, device=DEV))
+    _native.reset_counters()
+    for M, name in ((4, "mxfp4_rows"), (80, "mxfp4_gemm")):
+        x = torch.randn(M, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+        mxfp4_linear(x, w).sum().backward()
+        assert _native.counters().get(name) == 1
