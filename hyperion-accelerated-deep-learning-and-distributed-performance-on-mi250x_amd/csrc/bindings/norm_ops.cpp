@@ -183,6 +183,34 @@ void adam_mt(const at::Tensor& ptrs, const at::Tensor& sizes, const at::Tensor& 
                                        zero_grad ? 1 : 0));
 }
 
+void adam8_mt(const at::Tensor& ptrs, const at::Tensor& sizes, const at::Tensor& blocks, int64_t T, int64_t chunk,
+              double lr, double b1, double b2, double eps, double wd, bool adamw, const c10::optional<at::Tensor>& lr_t,
+              const at::Tensor& step_t, const c10::optional<at::Tensor>& inv_scale,
+              const c10::optional<at::Tensor>& found_inf, int64_t grad_dtype, int64_t param_dtype, bool zero_grad) {
+  TORCH_CHECK(sizes.numel() == T && ptrs.numel() == T * (param_dtype == hyp::kF32 ? 6 : 7),
+              "adam8_mt: table of 6 (low-precision parameters: 7) x T pointers and T sizes");
+  const at::DeviceGuard guard(ptrs.device());
+  HYP_CHECK_HIP(hyp::adam8_multi_tensor((int)grad_dtype, (int)param_dtype, ptrs.data_ptr<int64_t>(),
+                                        sizes.data_ptr<int64_t>(), blocks.data_ptr<int>(), (int)blocks.size(0), (int)T,
+                                        (int)chunk, (float)lr, b1, b2, (float)eps, wd, adamw ? 1 : 0,
+                                        ptr_or_null<float>(lr_t), step_t.data_ptr<float>(), ptr_or_null<float>(inv_scale),
+                                        ptr_or_null<float>(found_inf), cur_stream(), zero_grad ? 1 : 0));
+}
+
+// the moments of a table [m codes, v codes, m scales, v scales][T] as two dense fp32 vectors of `total` elements
+std::vector<at::Tensor> adam8_values(const at::Tensor& ptrs, const at::Tensor& sizes, const at::Tensor& blocks,
+                                     const at::Tensor& offs, int64_t T, int64_t chunk, int64_t total) {
+  TORCH_CHECK(sizes.numel() == T && ptrs.numel() == 4 * T && offs.numel() == T && offs.scalar_type() == at::kLong &&
+                  offs.device() == ptrs.device(), "adam8_values: table of 4 x T pointers, T sizes and T offsets");
+  const at::DeviceGuard guard(ptrs.device());
+  auto opt = at::TensorOptions().device(ptrs.device()).dtype(at::kFloat);
+  auto m = at::empty({total}, opt), v = at::empty({total}, opt);
+  HYP_CHECK_HIP(hyp::adam8_values(ptrs.data_ptr<int64_t>(), sizes.data_ptr<int64_t>(), blocks.data_ptr<int>(),
+                                  offs.data_ptr<int64_t>(), (int)blocks.size(0), (int)T, (int)chunk, m.data_ptr<float>(),
+                                  v.data_ptr<float>(), cur_stream()));
+  return {m, v};
+}
+
 void unscale_mt(const at::Tensor& ptrs, const at::Tensor& sizes, const at::Tensor& blocks, int64_t chunk,
                 const at::Tensor& inv_scale, const at::Tensor& found_inf, int64_t grad_dtype) {
   const at::DeviceGuard guard(ptrs.device());
@@ -244,6 +272,8 @@ void register_norm_ops(pybind11::module& m) {
         pybind11::arg("sums") = pybind11::none());
   m.def("bn_bwd_dx", &bn_bwd_dx, "BN backward dx pass from a pre-masked dz and its complete sums");
   m.def("adam_mt", &adam_mt, "multi-tensor fused Adam/AdamW");
+  m.def("adam8_mt", &adam8_mt, "multi-tensor fused Adam/AdamW with 8-bit moments");
+  m.def("adam8_values", &adam8_values, "8-bit moments of a table as dense fp32 vectors");
   m.def("adam_set_streaming", [](int64_t on) { hyp::adam_set_streaming((int)on); },
         "A/B: non-temporal loads / stores of the fp32 optimizer state in adam_mt");
   m.def("mse_fwd_bwd", [](const at::Tensor& x, const at::Tensor& t) {

@@ -43,6 +43,15 @@ hipError_t adam_multi_tensor(int grad_dtype, int param_dtype, const int64_t* ptr
                              const int* blocks, int nblocks, int T, int chunk, float lr, float b1, float b2, float eps,
                              float wd, int adamw, const float* lr_t, const float* step_t, const float* inv_scale,
                              const float* found_inf, hipStream_t stream, int zero_grad = 0);
+// ---- adam8.hip: moments in 8 bits, blocks of 256 elements.  ptrs = [param, grad, m codes (int8), v codes (uint8),
+// m scales, v scales] (+ fp32 master for kBF16 / kF16); chunk % 2048 == 0
+hipError_t adam8_multi_tensor(int grad_dtype, int param_dtype, const int64_t* ptrs, const int64_t* sizes,
+                              const int* blocks, int nblocks, int T, int chunk, float lr, double b1, double b2, float eps,
+                              double wd, int adamw, const float* lr_t, const float* step_t, const float* inv_scale,
+                              const float* found_inf, hipStream_t stream, int zero_grad = 0);
+// ptrs = [m codes, v codes, m scales, v scales]: the values of tensor t at offs[t] of the dense vectors m and v
+hipError_t adam8_values(const int64_t* ptrs, const int64_t* sizes, const int* blocks, const int64_t* offs, int nblocks,
+                        int T, int chunk, float* m, float* v, hipStream_t stream);
 hipError_t unscale_multi_tensor(int grad_dtype, const int64_t* ptrs, const int64_t* sizes, const int* blocks,
                                 int nblocks, int chunk, const float* inv_scale, float* found_inf, hipStream_t stream);
 hipError_t sumsq_multi_tensor(int grad_dtype, const int64_t* ptrs, const int64_t* sizes, const int* blocks, int nblocks,

@@ -12,6 +12,12 @@ state; the kernel updates the master and rewrites the compute copy in the same p
 model run its convolutions/GEMMs on bf16 weights directly (no per-forward autocast weight casts,
 no bf16→fp32 grad casts in backward) while the optimizer math stays in fp32.
 
+``state_bits=8`` holds the two moments in 8 bits (``csrc/kernels/adam8.hip``): 2 bytes and 8 bytes per
+256 elements instead of 8 bytes a parameter.  Blocks of 256 elements share an fp32 scale, the block's
+largest magnitude; the first moment is coded by the square root of its share of it, the second by the
+fourth root.  Everything else (masters, scalars on the device, skipped steps, the deferred clip) is as
+with 32 bits, and ``moment_vectors`` gives the values.
+
 Also provides multi-tensor global-norm clipping that takes the norm over *all* gradient shards
 (all-reduced when a process group is given) — the reference clipped only the local FSDP shard
 (``distributed_utils.py:351,522``).
@@ -20,7 +26,7 @@ from __future__ import annotations
 
 import math
 import weakref
-from typing import Iterable, List, Optional
+from typing import Iterable, List, Optional, Tuple
 
 import torch
 import torch.distributed as dist
@@ -47,6 +53,47 @@ def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.shape == b.shape and all(sa == sb for sa, sb, n in zip(a.stride(), b.stride(), a.shape) if n > 1)
 
 
+# ---- 8-bit moments (state_bits=8): the PyTorch path and oracle of adam8.hip ------------------------
+STATE_BLOCK = 256  # elements that share a scale (adam8.hip)
+_STATE8 = ("exp_avg_q", "exp_avg_sq_q", "exp_avg_scale", "exp_avg_sq_scale")
+
+
+def _channels_last(p: torch.Tensor) -> bool:
+    return p.dim() == 4 and not p.is_contiguous() and p.is_contiguous(memory_format=torch.channels_last)
+
+
+def _memory_order(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    """``t`` flat in the order that the blocks of ``like``'s moments follow: its memory order (channels-last
+    4-D parameters), else row-major.  A view where the layout allows it."""
+    return (t.permute(0, 2, 3, 1) if _channels_last(like) else t).reshape(-1)
+
+
+def _in_blocks(x: torch.Tensor) -> torch.Tensor:
+    return torch.nn.functional.pad(x, (0, -x.numel() % STATE_BLOCK)).view(-1, STATE_BLOCK)
+
+
+def _encode8(x: torch.Tensor, levels: int, second: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp64 [n] -> (codes [n], fp32 scales)"""
+    b = _in_blocks(x)
+    s = b.abs().amax(1).float() if b.numel() else b.new_zeros(0).float()
+    s = torch.where(s < torch.finfo(torch.float32).tiny, torch.zeros_like(s), s)
+    s = torch.where(torch.isfinite(s), s, torch.full_like(s, math.nan))
+    live = (s > 0)[:, None]
+    r = torch.where(live, b.abs() / s.double()[:, None], torch.zeros_like(b)).sqrt()
+    q = torch.round((r.sqrt() if second else r) * levels).clamp(max=levels)
+    if second:
+        q = torch.where(live & (b > 0) & (q < 1), torch.ones_like(q), q)
+    else:
+        q = torch.where(b < 0, -q, q)
+    return q.to(torch.uint8 if second else torch.int8).view(-1)[:x.numel()], s
+
+
+def _decode8(q: torch.Tensor, s: torch.Tensor, levels: int, second: bool) -> torch.Tensor:
+    b = _in_blocks(q.double())
+    b = b * b * (b * b if second else torch.sign(b))
+    return (b * (s.double() / float(levels) ** (4 if second else 2))[:, None]).view(-1)[:q.numel()]
+
+
 class FusedAdam(torch.optim.Optimizer):
     def __init__(
         self,
@@ -57,10 +104,17 @@ class FusedAdam(torch.optim.Optimizer):
         weight_decay: float = 0.0,
         adamw: bool = False,
         zero_grad_in_step: bool = False,
+        state_bits: int = 32,
     ):
         """``zero_grad_in_step``: the kernel writes zeros over each gradient as it consumes it, so
         ``zero_grad(set_to_none=False)`` before the next backward is free (one fill kernel per
-        parameter saved — 256 launches per step for Llama LoRA under hipGraph capture)."""
+        parameter saved — 256 launches per step for Llama LoRA under hipGraph capture).
+        ``state_bits``: 32 (fp32 moments) or 8 (coded moments, module docstring)."""
+        if state_bits not in (8, 32):
+            raise ValueError(f"FusedAdam: state_bits must be 8 or 32, got {state_bits}")
+        if state_bits == 8 and not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"FusedAdam: betas must be in [0, 1), got {betas}")
+        self.state_bits = state_bits
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, adamw=adamw)
         super().__init__(params, defaults)
         self.zero_grad_in_step = zero_grad_in_step
@@ -76,6 +130,14 @@ class FusedAdam(torch.optim.Optimizer):
 
     def _state(self, p: torch.Tensor):
         st = self.state[p]
+        if not st and self.state_bits == 8:
+            n, nb = p.numel(), -(-p.numel() // STATE_BLOCK)
+            st["exp_avg_q"] = torch.zeros(n, dtype=torch.int8, device=p.device)
+            st["exp_avg_sq_q"] = torch.zeros(n, dtype=torch.uint8, device=p.device)
+            st["exp_avg_scale"] = torch.zeros(nb, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq_scale"] = torch.zeros(nb, dtype=torch.float32, device=p.device)
+            if p.dtype != torch.float32:
+                st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format).clone()
         if not st:
             st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
             st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
@@ -117,6 +179,9 @@ class FusedAdam(torch.optim.Optimizer):
             for (pdt, gdt), ps in parts.items():
                 sts = [self._state(p) for p in ps]
                 gs = [grad_of(p) for p in ps]
+                if self.state_bits == 8:
+                    self._step8(f"adam8_{gi}_{pdt}_{gdt}", group, ps, gs, sts, inv_scale, native)
+                    continue
                 ms = [s["exp_avg"] for s in sts]
                 vs = [s["exp_avg_sq"] for s in sts]
                 masters = [s["master"] for s in sts] if pdt != torch.float32 else None
@@ -147,6 +212,102 @@ class FusedAdam(torch.optim.Optimizer):
                         for g in gs:
                             g.zero_()
         return loss
+
+    def _step8(self, role, group, ps, gs, sts, inv_scale, native):
+        """One partition (a parameter dtype and a gradient dtype) with 8-bit moments."""
+        pdt, gdt = ps[0].dtype, gs[0].dtype
+        master = pdt != torch.float32
+        ok = native and pdt in _native.DTYPE_CODE and gdt in _native.DTYPE_CODE and all(
+            _dense(p) and _dense(g) and _same_layout(p, g) for p, g in zip(ps, gs))
+        if ok:
+            groups = [ps, gs] + [[s[k] for s in sts] for k in _STATE8]
+            if master:
+                groups.append([s["master"] for s in sts])
+            try:
+                tab = self._tables.get(role, groups)
+            except ValueError:  # misaligned tensor -> reference path
+                ok = False
+        if ok:
+            lr = group["lr"]
+            lr_t = lr if isinstance(lr, torch.Tensor) else None
+            b1, b2 = group["betas"]
+            _native.count("adam8")
+            _native.native().adam8_mt(
+                tab.ptrs, tab.sizes, tab.blocks, tab.T, tab.chunk, float(lr) if lr_t is None else 0.0, b1, b2,
+                group["eps"], group["weight_decay"], bool(group["adamw"]), lr_t, self._step_t, inv_scale, self.found_inf,
+                _native.DTYPE_CODE[gdt], _native.DTYPE_CODE[pdt], bool(self.zero_grad_in_step))
+            return
+        self._reference_step8(group, ps, gs, sts, inv_scale)
+        if self.zero_grad_in_step:
+            for g in gs:
+                g.zero_()
+
+    def _reference_step8(self, group, ps, gs, sts, inv_scale=None):
+        """PyTorch reference of the 8-bit step (CPU / fallback): moments and codes in fp64."""
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdam: reference path reached during hipGraph capture (grad/param layouts "
+                               "or dtypes outside the fused kernel's envelope)")
+        if self.found_inf is not None and float(self.found_inf) != 0.0:
+            return
+        b1, b2 = group["betas"]
+        lr, wd, eps = float(group["lr"]), group["weight_decay"], group["eps"]
+        bc1, bc2_sqrt = 1 - b1**self._host_step, math.sqrt(1 - b2**self._host_step)
+        inv = float(inv_scale) if inv_scale is not None else 1.0
+        for p, g, st in zip(ps, gs, sts):
+            w = st.get("master", p)
+            flat = _memory_order(w, p).float()
+            g = (_memory_order(g, p).float() * inv).double()
+            if group["adamw"]:
+                flat = flat * (1 - lr * wd)
+            elif wd != 0:
+                g = g + flat.double() * wd
+            m = _decode8(st["exp_avg_q"], st["exp_avg_scale"], 127, False) * b1 + g * (1 - b1)
+            v = _decode8(st["exp_avg_sq_q"], st["exp_avg_sq_scale"], 255, True) * b2 + g * g * (1 - b2)
+            flat = (flat.double() - lr / bc1 * (m / (v.sqrt() / bc2_sqrt + eps))).float()
+            for x, levels, second, key in ((m, 127, False, "exp_avg"), (v, 255, True, "exp_avg_sq")):
+                q, s = _encode8(x, levels, second)
+                st[key + "_q"].copy_(q)
+                st[key + "_scale"].copy_(s)
+            if _channels_last(p):
+                flat = flat.view(p.shape[0], p.shape[2], p.shape[3], p.shape[1]).permute(0, 3, 1, 2)
+            w.copy_(flat.view(p.shape) if not _channels_last(p) else flat)
+            if w is not p:
+                p.copy_(w)
+
+    @torch.no_grad()
+    def moment_vectors(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The first and second moments of every parameter that has been stepped, as two fp32 vectors: the
+        parameters in order, each row-major (like ``torch.nn.utils.parameters_to_vector``)."""
+        ps = [p for g in self.param_groups for p in g["params"] if self.state.get(p)]
+        sts = [self.state[p] for p in ps]
+        if not ps:
+            return torch.zeros(0), torch.zeros(0)
+        if self.state_bits == 32:
+            return tuple(torch.cat([s[k].reshape(-1) for s in sts]) for k in ("exp_avg", "exp_avg_sq"))
+        sizes = [p.numel() for p in ps]
+        tab = None
+        if _native.use_native(*ps, op="adam") and all(p.device == ps[0].device for p in ps):
+            try:
+                tab = self._tables.get("adam8_values", [[s[k] for s in sts] for k in _STATE8])
+            except ValueError:
+                pass
+        if tab is not None:
+            offs = getattr(tab, "offs", None)
+            if offs is None:
+                starts = torch.tensor([0] + sizes[:-1]).cumsum(0)
+                offs = tab.offs = starts.to(ps[0].device)
+            m, v = _native.native().adam8_values(tab.ptrs, tab.sizes, tab.blocks, offs, tab.T, tab.chunk, sum(sizes))
+        else:
+            m = torch.cat([_decode8(s["exp_avg_q"], s["exp_avg_scale"], 127, False).float() for s in sts])
+            v = torch.cat([_decode8(s["exp_avg_sq_q"], s["exp_avg_sq_scale"], 255, True).float() for s in sts])
+        at = 0
+        for p, n in zip(ps, sizes):
+            if _channels_last(p):  # coded in memory order
+                for x in (m, v):
+                    nhwc = x[at:at + n].view(p.shape[0], p.shape[2], p.shape[3], p.shape[1])
+                    x[at:at + n] = nhwc.permute(0, 3, 1, 2).reshape(-1)
+            at += n
+        return m, v
 
     def _reference_step(self, group, ps, gs, ms, vs, masters=None, inv_scale=None):
         """PyTorch reference (CPU / fallback); identical math to the kernel."""
@@ -182,17 +343,50 @@ class FusedAdam(torch.optim.Optimizer):
         sd["hyperion_step"] = self._host_step
         return sd
 
+    def _check_state(self, st, p):
+        """Refuses a saved state of the other kind, and 8-bit moments that do not fit: the kernels trust their
+        types and sizes."""
+        if self.state_bits == 32:
+            if "exp_avg_q" in st:
+                raise ValueError("FusedAdam(state_bits=32): the saved state has 8-bit moments (state_bits=8)")
+            return
+        n, nb = p.numel(), -(-p.numel() // STATE_BLOCK)
+        want = {"exp_avg_q": (torch.int8, n), "exp_avg_sq_q": (torch.uint8, n),
+                "exp_avg_scale": (torch.float32, nb), "exp_avg_sq_scale": (torch.float32, nb)}
+        if p.dtype != torch.float32:
+            want["master"] = (torch.float32, n)
+        for k, (dt, size) in want.items():
+            t = st.get(k)
+            if not isinstance(t, torch.Tensor) or t.dtype != dt or t.numel() != size:
+                raise ValueError(f"FusedAdam(state_bits=8): the saved state of a {tuple(p.shape)} {p.dtype} parameter needs "
+                                 f"{k!r} with {size} elements of {dt}, got {None if t is None else (tuple(t.shape), t.dtype)}")
+
     def load_state_dict(self, state_dict):
         state_dict = dict(state_dict)
-        self._host_step = int(state_dict.pop("hyperion_step", 0))
+        host_step = int(state_dict.pop("hyperion_step", 0))
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        if len(saved) == len(own):  # (else the base class refuses)
+            for i, p in zip(saved, own):
+                if state_dict["state"].get(i):
+                    self._check_state(state_dict["state"][i], p)
         super().load_state_dict(state_dict)
+        self._host_step = host_step
+        # the base class casts every state tensor to its parameter's dtype: moments and masters of bf16 / fp16
+        # parameters are fp32, codes are integers, and the kernels read them as such
+        for i, p in zip(saved, own):
+            for k, t in state_dict["state"].get(i, {}).items():
+                if k in _STATE8:
+                    self.state[p][k] = t.detach().to(p.device).reshape(-1).clone()
+                elif k in ("exp_avg", "exp_avg_sq", "master"):
+                    self.state[p][k] = t.detach().to(p.device, torch.float32).clone()
         self._step_t = None
         # the table cache is kept: tables a captured graph uses stay pinned; new state tensors
         # simply key new tables
 
 
-def FusedAdamW(params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
-    return FusedAdam(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, adamw=True)
+def FusedAdamW(params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+    return FusedAdam(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, adamw=True, state_bits=state_bits)
 
 
 # clip tables per model: keyed (weakly) by the first parameter, so two same-shaped models never

@@ -1,0 +1,130 @@
+"""adam8 kernels against the 64-bit oracle: types, odd sizes, layouts, skipped steps, graphs, streams."""
+import pytest
+import torch
+
+from hyperion.ops import FusedAdam, FusedAdamW, _native, clip_grad_norm_
+
+from test_adam8_cpu import run_against_oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SHAPES = [(3, 5), (256,), (257,), (1,), (40, 33), (8192,), (8193,), (130, 777), (2047,)]
+
+
+@pytest.mark.parametrize("gdtype", [None, torch.float32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("adamw", [True, False])
+def test_steps_against_oracle(dtype, gdtype, adamw):
+    _native.reset_counters()
+    if gdtype is None:
+        run_against_oracle(SHAPES, dtype, DEV, adamw=adamw)
+    else:  # gradients scaled by the loss scaler's factor
+        run_against_oracle(SHAPES, dtype, DEV, adamw=adamw, scale=2.0 ** -7)
+    assert _native.counters()["adam8"] == 4
+
+
+def test_without_weight_decay_and_channels_last():
+    run_against_oracle([(5, 7, 3, 3), (64, 64, 3, 3), (9,)], torch.float32, DEV, adamw=False, wd=0.0, layout=torch.channels_last)
+
+
+def test_same_codes_as_the_cpu():
+    torch.manual_seed(0)
+    w = torch.randn(100, 300)
+    ps = [torch.nn.Parameter(w.clone().to(d)) for d in ("cpu", DEV)]
+    opts = [FusedAdamW([p], lr=1e-2, state_bits=8) for p in ps]
+    for _ in range(5):
+        g = torch.randn(100, 300)
+        for p, o in zip(ps, opts):
+            p.grad = g.to(p.device)
+            o.step()
+        a, b = (o.state[p] for p, o in zip(ps, opts))
+        for k in ("exp_avg_q", "exp_avg_sq_q", "exp_avg_scale", "exp_avg_sq_scale"):
+            assert torch.equal(a[k], b[k].cpu()), k
+
+
+def test_zero_and_non_finite_blocks():
+    p = torch.nn.Parameter(torch.ones(600, device=DEV))
+    opt = FusedAdamW([p], lr=0.1, state_bits=8, weight_decay=0.0)
+    p.grad = torch.zeros(600, device=DEV)
+    p.grad[300] = float("inf")
+    p.grad[599] = 1e-30
+    opt.step()
+    m, v = opt.moment_vectors()
+    assert (m[:256] == 0).all() and torch.isnan(m[256:512]).all() and torch.isnan(v[256:512]).all()
+    assert m[599] != 0 and v[599] == 0 and (v[512:] == 0).all()
+    assert torch.isfinite(p.detach()[:256]).all() and torch.isfinite(p.detach()[301:]).all()
+
+
+def test_skipped_step_zeroed_gradients_and_deferred_clip():
+    p = torch.nn.Parameter(torch.ones(1000, device=DEV))
+    opt = FusedAdamW([p], state_bits=8)
+    opt.zero_grad_in_step = True
+    opt.found_inf = torch.ones(1, device=DEV)
+    p.grad = torch.ones(1000, device=DEV)
+    opt.step()
+    assert (p == 1).all() and (p.grad == 0).all() and (opt.moment_vectors()[0] == 0).all()
+    opt.found_inf = torch.zeros(1, device=DEV)
+    p.grad.fill_(2.0)
+    clip_grad_norm_([p], 1.0, defer_to=opt)
+    opt.step()
+    want = 0.1 * 2.0 / (2.0 * 1000 ** 0.5 + 1e-6)
+    assert (p.grad == 0).all()
+    torch.testing.assert_close(opt.moment_vectors()[0], torch.full((1000,), want, device=DEV), rtol=1e-5, atol=0)
+
+
+def test_misaligned_parameters_take_the_torch_path():
+    buf = torch.randn(301, device=DEV)
+    p = torch.nn.Parameter(buf[1:])
+    q = torch.nn.Parameter(buf[1:].clone())
+    a, b = FusedAdamW([p], state_bits=8), FusedAdamW([q], state_bits=8)
+    for _ in range(3):
+        g = torch.randn(300, device=DEV)
+        p.grad, q.grad = g.clone(), g.clone()
+        a.step(), b.step()
+    assert all(torch.equal(a.state[p][k], b.state[q][k]) for k in ("exp_avg_q", "exp_avg_sq_q"))
+    torch.testing.assert_close(p, q, rtol=1e-6, atol=1e-7)
+
+
+def test_other_stream_and_graph_replays():
+    torch.manual_seed(2)
+    ws = [torch.randn(300, 70, device=DEV).bfloat16(), torch.randn(9001, device=DEV).bfloat16()]
+    grads = [[torch.randn_like(w) for w in ws] for _ in range(7)]
+    pairs = []
+    for _ in range(2):
+        ps = [torch.nn.Parameter(w.clone()) for w in ws]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        pairs.append((ps, FusedAdamW(ps, lr=1e-2, state_bits=8)))
+
+    def load(ps, i):
+        for p, g in zip(ps, grads[i]):
+            p.grad.copy_(g)
+
+    (pa, oa), (pb, ob) = pairs
+    s = torch.cuda.Stream()
+    for i in range(2):
+        load(pa, i)
+        oa.step()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            load(pb, i)
+            ob.step()
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ob.step()
+        values = ob.moment_vectors() if "adam8_values" in ob._tables._tables else None
+    for i in range(2, 7):
+        load(pa, i)
+        oa.step()
+        load(pb, i)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(pa, pb))
+        assert all(torch.equal(x, y) for x, y in zip(oa.moment_vectors(), ob.moment_vectors()))
+    assert values is None
+
+
+def test_many_small_tensors_in_one_launch():
+    run_against_oracle([(17, i % 9 + 1) for i in range(120)], torch.bfloat16, DEV, steps=2)
