@@ -36,6 +36,7 @@ from ..ops.layernorm import RMSNorm
 from ..ops.linear import Linear as HypLinear
 from ..ops.rope import apply_rope
 from ..ops.swiglu import swiglu
+from ..ops.token_logprobs import TokenLogprobs, token_logprobs
 
 
 # HYPERION_LLAMA_FUSED=0 keeps every layer on the module path (A/B runs, numerics tests)
@@ -234,6 +235,14 @@ class LlamaForCausalLM(nn.Module):
         if return_logits or (return_logits is None and labels is None):
             out["logits"] = self.lm_head(h)
         return out
+
+    def token_logprobs(self, input_ids: torch.Tensor, labels: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
+                       top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+        """Scores of ``labels[:, 1:]`` given the tokens before each (-100 is ignored), [B, S - 1]: what a
+        preference or policy objective, or a perplexity by position, is made of (differentiable)."""
+        h = self.model(input_ids, attention_mask)
+        return token_logprobs(self.lm_head(h[:, :-1]), labels[:, 1:], top_k=top_k, ignore_index=-100,
+                              temperature=temperature)
 
 
 def llama2_7b(**kw) -> LlamaForCausalLM:

@@ -13,18 +13,26 @@ prefixed ``base_model.model.``) that ``PeftModel.from_pretrained`` reads.
 Compute: ``y = x Wᵀ (+ b) + s · (drop(x) Aᵀ) Bᵀ`` through ``ops.lora.lora_linear`` — the frozen
 base GEMM plus the low-rank update with the dropout mask regenerated from a seed in backward
 (never stored), and no gradient buffer ever allocated for W.
+
+``apply_lora(..., base_format="mxfp4")`` (or :func:`quantize_base`) holds the frozen linear layers in 4
+bits (``ops.mxfp4``): 17/64 of the bf16 base's memory and weight stream; the adapters, their files and
+their keys stay as they are.
 """
 from __future__ import annotations
 
 import json
 import math
 import os
-from typing import Dict, Iterable, List
+from typing import Dict, Iterable, List, Optional
 
 import torch
 import torch.nn as nn
 
+from ..ops.cross_entropy import LinearCrossEntropy
+from ..ops.dropout import dropout
+from ..ops.linear import linear
 from ..ops.lora import lora_linear
+from ..ops.mxfp4 import MXFP4Linear, MXFP4Tensor
 
 
 class LoRALinear(nn.Module):
@@ -55,6 +63,9 @@ class LoRALinear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         a = self.adapter
         p = self.p if self.training else 0.0
+        if isinstance(self.base_layer, MXFP4Linear):
+            t = linear(dropout(x, p, self.training), self.lora_A[a].weight)
+            return self.base_layer(x) + self.scaling[a] * linear(t, self.lora_B[a].weight)
         return lora_linear(x, self.base_layer.weight, self.base_layer.bias, self.lora_A[a].weight,
                            self.lora_B[a].weight, self.scaling[a], p)
 
@@ -62,13 +73,19 @@ class LoRALinear(nn.Module):
     def merged_weight(self) -> torch.Tensor:
         a = self.adapter
         dw = (self.lora_B[a].weight.float() @ self.lora_A[a].weight.float()) * self.scaling[a]
-        return (self.base_layer.weight.float() + dw).to(self.base_layer.weight.dtype)
+        w = self.base_layer.weight
+        if isinstance(w, MXFP4Tensor):
+            return (w.dequantize(torch.float32) + dw).to(self.lora_A[a].weight.dtype)
+        return (w.float() + dw).to(w.dtype)
 
 
 def apply_lora(model: nn.Module, r: int = 16, alpha: float = 32.0, dropout: float = 0.05,
                target_modules: Iterable[str] = ("q_proj", "k_proj", "v_proj", "o_proj"),
-               adapter: str = "default") -> nn.Module:
-    """Freeze every parameter and wrap target ``nn.Linear``s in :class:`LoRALinear` (in place)."""
+               adapter: str = "default", base_format: Optional[str] = None) -> nn.Module:
+    """Freeze every parameter and wrap target ``nn.Linear``s in :class:`LoRALinear` (in place).
+    ``base_format="mxfp4"`` then holds the frozen linear layers in 4 bits (:func:`quantize_base`)."""
+    if base_format not in (None, "mxfp4"):
+        raise ValueError(f"apply_lora: base_format must be None or 'mxfp4', got {base_format!r}")
     targets = set(target_modules)
     for p in model.parameters():
         p.requires_grad_(False)
@@ -77,6 +94,19 @@ def apply_lora(model: nn.Module, r: int = 16, alpha: float = 32.0, dropout: floa
             if cname in targets and isinstance(child, nn.Linear) and not isinstance(child, LoRALinear):
                 setattr(mod, cname, LoRALinear(child, r, alpha, dropout, adapter))
     model.peft_config = {adapter: lora_config_dict(r, alpha, dropout, sorted(targets))}
+    return quantize_base(model) if base_format == "mxfp4" else model
+
+
+def quantize_base(model: nn.Module) -> nn.Module:
+    """Hold every frozen linear layer (a LoRA layer's base among them) in 4 bits, in place.  LM heads
+    (``LinearCrossEntropy``) and layers with trainable weights stay as they are."""
+    adapters = {id(m) for lora in model.modules() if isinstance(lora, LoRALinear)
+                for d in (lora.lora_A, lora.lora_B) for m in d.values()}
+    for mod in list(model.modules()):
+        for cname, child in list(mod.named_children()):
+            if (isinstance(child, nn.Linear) and not isinstance(child, LinearCrossEntropy)
+                    and not child.weight.requires_grad and id(child) not in adapters):
+                setattr(mod, cname, MXFP4Linear.from_linear(child))
     return model
 
 
@@ -139,7 +169,15 @@ def merge_lora(model: nn.Module) -> nn.Module:
         for cname, child in list(mod.named_children()):
             if isinstance(child, LoRALinear):
                 base = child.base_layer
-                base.weight.data.copy_(child.merged_weight())
+                if isinstance(base, MXFP4Linear):  # the merged weight is no 4-bit one any more
+                    w = child.merged_weight()
+                    full = nn.Linear(base.in_features, base.out_features, bias=False, device=w.device, dtype=w.dtype)
+                    full.weight.data.copy_(w)
+                    full.weight.requires_grad_(False)
+                    full.bias = base.bias
+                    base = full
+                else:
+                    base.weight.data.copy_(child.merged_weight())
                 setattr(mod, cname, base)
     return model
 

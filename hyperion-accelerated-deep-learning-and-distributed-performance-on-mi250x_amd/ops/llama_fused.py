@@ -120,7 +120,7 @@ def _fuse_layer(m: nn.Module) -> int:
     n = 0
     for mods in ((at.q_proj, at.k_proj, at.v_proj), (mlp.gate_proj, mlp.up_proj)):
         ws = [_base_weight(x) for x in mods]
-        if any(w.requires_grad for w in ws) or _adjacent(ws):
+        if any(not isinstance(w, torch.Tensor) or w.requires_grad for w in ws) or _adjacent(ws):
             continue
         with torch.no_grad():
             buf = torch.cat([w.detach() for w in ws], 0)
@@ -173,8 +173,8 @@ def fused_spec(layer: nn.Module, x: torch.Tensor, kpm: Optional[torch.Tensor]) -
     at, mlp = layer.self_attn, layer.mlp
     qkv = [at.q_proj, at.k_proj, at.v_proj]
     ws = [_base_weight(m) for m in qkv + [at.o_proj, mlp.gate_proj, mlp.up_proj, mlp.down_proj]]
-    if any(w.requires_grad or w.dtype != x.dtype for w in ws):
-        return None
+    if any(not isinstance(w, torch.Tensor) or w.requires_grad or w.dtype != x.dtype for w in ws):
+        return None  # (a 4-bit base runs on the module path)
     if (layer.input_layernorm.weight.requires_grad or layer.post_attention_layernorm.weight.requires_grad
             or any(hasattr(m, "lora_A") for m in (mlp.gate_proj, mlp.up_proj, mlp.down_proj))):
         return None

@@ -609,7 +609,7 @@ def train_llama_fsdp(rank: int, world: int, *, epochs: int = 1, base_dir: str = 
                      hf_token: Optional[str] = None, model_id: str = "NousResearch/Llama-2-7b-hf", lora: bool = False,
                      batch_size: int = 1, progress_every: int = 50, opts: Optional[RunOptions] = None,
                      config=None, lora_parallel: str = "fsdp", mask_pad_labels: bool = False,
-                     replicate_frozen="auto") -> Dict:
+                     replicate_frozen="auto", base_format: Optional[str] = None, state_bits: int = 32) -> Dict:
     """C26: Llama fine-tune.  ``lora=True``: frozen bf16 base + r16 adapters on q/k/v/o.
 
     ``lora_parallel='fsdp'`` (default; the BASELINE.json config) wraps the model in FSDP with one
@@ -627,7 +627,11 @@ def train_llama_fsdp(rank: int, world: int, *, epochs: int = 1, base_dir: str = 
     ``replicate_frozen`` ("auto" | True | False): under FSDP keep the frozen base whole on every rank
     when it fits (auto: <= 1/4 of HBM — 13.5 GB of 288 GB on MI355X), so only the adapters are
     sharded and communicated; False shards the base like the reference's torch FSDP.
+    ``base_format="mxfp4"`` (with ``lora``, on one GPU or under DDP) holds the frozen base in 4 bits;
+    ``state_bits=8`` the optimizer's moments in 8.
     """
+    if base_format is not None and not (lora and (lora_parallel == "ddp" or world == 1)):
+        raise ValueError("train_llama_fsdp: base_format needs lora=True on one GPU or with lora_parallel='ddp'")
     from ..models.llama import LlamaConfig, LlamaDecoderLayer, LlamaForCausalLM
     from ..models.lora import apply_lora, save_adapter
     from ..parallel.ddp import DDP
@@ -655,8 +659,8 @@ def train_llama_fsdp(rank: int, world: int, *, epochs: int = 1, base_dir: str = 
     elif rank == 0 and model_id and not os.path.isdir(str(model_id)):
         opts.log(f"[llama] {model_id}: not a local HF checkpoint directory -> random-init weights")
     if lora:
-        base = apply_lora(base, r=16, alpha=32, dropout=0.05)
-        mode = f"lora_{precision}"
+        base = apply_lora(base, r=16, alpha=32, dropout=0.05, base_format=base_format)
+        mode = f"lora_{precision}" + (f"_{base_format}" if base_format else "")
     else:
         mode = f"fsdp_{precision}"
     policy = transformer_auto_wrap_policy({LlamaDecoderLayer})
@@ -666,7 +670,8 @@ def train_llama_fsdp(rank: int, world: int, *, epochs: int = 1, base_dir: str = 
     else:
         model = FSDP(base, auto_wrap_policy=policy, device_id=device, mixed_precision=MixedPrecision(pdt, pdt, pdt),
                      replicate_frozen=replicate_frozen if lora else False, ring=opts.fsdp_ring)
-    opt = FusedAdam([p for p in model.parameters() if p.requires_grad], lr=1e-5, weight_decay=0.01, adamw=True)
+    opt = FusedAdam([p for p in model.parameters() if p.requires_grad], lr=1e-5, weight_decay=0.01, adamw=True,
+                    state_bits=state_bits)
     runner = _EpochRunner(rank, world, device, model, opt, None, None, 1.0, isinstance(model, FSDP), opts)
     res = _maybe_resume(opts, model, opt, None, out, "llama")
     run_id = res.run_id or _shared_run_id("llama", world)

@@ -1,0 +1,58 @@
+"""LoRA on a 4-bit base, token log probabilities and 8-bit AdamW together, on the CPU paths."""
+import pytest
+import torch
+
+from hyperion.models.lora import LoRALinear, apply_lora, load_adapter, merge_lora, quantize_base, save_adapter
+from hyperion.models.llama import LlamaConfig, LlamaForCausalLM
+from hyperion.ops.mxfp4 import MXFP4Linear
+
+from lean_finetune import batch, build, check_step, dequantized
+
+
+def test_step_against_the_dequantised_model():
+    # fp32 on both sides: sums of up to 512 terms in two orders, through two layers
+    check_step("cpu", torch.float32, 1e-4)
+
+
+def test_keys_adapters_and_merge(tmp_path):
+    m = build("cpu", torch.float32)
+    keys = set(m.state_dict())
+    assert "model.layers.0.self_attn.q_proj.base_layer.weight_codes" in keys and "lm_head.weight" in keys
+    assert "model.layers.0.mlp.up_proj.weight_scales" in keys
+    save_adapter(m, str(tmp_path))
+    plain = apply_lora(LlamaForCausalLM(LlamaConfig.tiny(num_key_value_heads=1)), r=8, alpha=16, dropout=0.0)
+    load_adapter(plain, str(tmp_path))  # the adapter files are those of any base
+    for a, b in zip([x for x in m.modules() if isinstance(x, LoRALinear)], [x for x in plain.modules() if isinstance(x, LoRALinear)]):
+        assert torch.equal(a.lora_B["default"].weight, b.lora_B["default"].weight)
+    ids, mask, _, _ = batch("cpu")
+    m.eval()
+    want = m(ids, mask).logits
+    merged = merge_lora(m)
+    assert not any(isinstance(x, LoRALinear) for x in merged.modules())
+    torch.testing.assert_close(merged(ids, mask).logits, want, atol=1e-4, rtol=1e-4)
+
+
+def test_dropout_and_refusals():
+    m = build("cpu", torch.float32)
+    layer = next(x for x in m.modules() if isinstance(x, LoRALinear))
+    layer.p = 0.5
+    x = torch.randn(4, 128)
+    torch.manual_seed(0)
+    a = layer.train()(x)
+    assert not torch.equal(a, layer.eval()(x))
+    with pytest.raises(ValueError):
+        apply_lora(LlamaForCausalLM(LlamaConfig.tiny()), base_format="int3")
+    trainable = LlamaForCausalLM(LlamaConfig.tiny())
+    assert not any(isinstance(x, MXFP4Linear) for x in quantize_base(trainable).modules())
+    assert dequantized(m) is not m
+
+
+def test_trainer_with_a_4_bit_base(tmp_path):
+    from hyperion.train.distributed import train_llama_fsdp
+    from test_trainers_cpu import _opts
+
+    r = train_llama_fsdp(0, 1, epochs=1, base_dir=str(tmp_path), lora=True, batch_size=2, progress_every=0, opts=_opts(),
+                         config=LlamaConfig.tiny(num_hidden_layers=1), base_format="mxfp4", state_bits=8)
+    assert r["history"][0]["steps"] == 2 and r["mode"].endswith("mxfp4")
+    with pytest.raises(ValueError, match="base_format"):
+        train_llama_fsdp(0, 1, base_dir=str(tmp_path), lora=False, base_format="mxfp4")
