@@ -43,55 +43,132 @@ at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, int6
 
 int pieces_of(at::ScalarType t) { return t == at::kBFloat16 ? 1 : (t == at::kHalf ? 2 : 3); }
 
-// x [R, K] (unit stride in K) as bf16 pieces [P R, pitch], zeros behind K
-at::Tensor mx_pieces(const at::Tensor& x, int64_t pitch) {
-  HYP_CHECK_CUDA_TENSOR(x);
-  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1) && pitch % 8 == 0 && pitch >= x.size(1) &&
-                  pitch < (int64_t)INT32_MAX, "mx_pieces: x [R, K] with unit stride in K, pitch >= K a multiple of 8");
-  const at::DeviceGuard guard(x.device());
-  const int P = pieces_of(x.scalar_type());
-  auto out = at::empty({P * x.size(0), pitch}, x.options().dtype(at::kBFloat16));
+const float* bias_ptr(const c10::optional<at::Tensor>& bias, int64_t n, const at::Device& dev, const char* who) {
+  if (!bias.has_value() || !bias->defined()) return nullptr;
+  TORCH_CHECK(bias->scalar_type() == at::kFloat && bias->is_contiguous() && bias->numel() == n && bias->device() == dev &&
+                  reinterpret_cast<uintptr_t>(bias->data_ptr()) % 16 == 0,
+              who, ": bias must be a contiguous, 16-byte aligned fp32 [", n, "]");
+  return bias->data_ptr<float>();
+}
+
+// x [M, n] (unit stride in n) as bf16 pieces [P M, pitch] whose sum it is, zeros behind n; x itself where it is that
+at::Tensor pieces(const at::Tensor& x, int64_t pitch) {
+  if (x.scalar_type() == at::kBFloat16 && x.size(1) == pitch && x.is_contiguous() &&
+      reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0)
+    return x;
+  auto out = at::empty({pieces_of(x.scalar_type()) * x.size(0), pitch}, x.options().dtype(at::kBFloat16));
   HYP_CHECK_HIP(hyp::mx_pieces(dtype_code(x), x.data_ptr(), x.stride(0), x.size(0), (int)x.size(1), (int)pitch,
                                out.data_ptr(), cur_stream()));
   return out;
 }
 
-const float* bias_ptr(const c10::optional<at::Tensor>& bias, int64_t n, const at::Device& dev, const char* who) {
-  if (!bias.has_value() || !bias->defined()) return nullptr;
-  TORCH_CHECK(bias->scalar_type() == at::kFloat && bias->is_contiguous() && bias->numel() == n && bias->device() == dev,
-              who, ": bias must be a contiguous fp32 [", n, "]");
-  return bias->data_ptr<float>();
-}
-
-// sum over the pieces of part [P R, pitch] (fp32), columns [0, cols), + bias -> [R, cols] in dtype
-at::Tensor mx_join(const at::Tensor& part, int64_t rows, int64_t cols, const c10::optional<at::Tensor>& bias,
-                   at::ScalarType dtype) {
-  HYP_CHECK_CUDA_TENSOR(part);
-  TORCH_CHECK(part.scalar_type() == at::kFloat && part.dim() == 2 && part.is_contiguous() && part.size(1) >= cols &&
-                  rows > 0 && part.size(0) % rows == 0, "mx_join: contiguous fp32 part [P * rows, >= cols]");
-  const at::DeviceGuard guard(part.device());
-  auto y = at::empty({rows, cols}, part.options().dtype(dtype));
-  HYP_CHECK_HIP(hyp::mx_join(dtype_code(dtype), part.data_ptr<float>(), (int)(part.size(0) / rows), rows, (int)cols,
-                             part.size(1), bias_ptr(bias, cols, part.device(), "mx_join"), y.data_ptr(), cur_stream()));
+// sum over the pieces of part [P M, pitch] (fp32), columns [0, cols), + bias -> [M, cols] in dtype
+at::Tensor join(const at::Tensor& part, int64_t M, int64_t cols, const float* bias, at::ScalarType dtype) {
+  auto y = at::empty({M, cols}, part.options().dtype(dtype));
+  HYP_CHECK_HIP(hyp::mx_join(dtype_code(dtype), part.data_ptr<float>(), (int)(part.size(0) / M), M, (int)cols, part.size(1),
+                             bias, y.data_ptr(), cur_stream()));
   return y;
 }
 
-// x [M, 32 nb] bf16 contiguous times the weight's transpose -> [M, N] (bf16 or fp32)
-at::Tensor mx_rows(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
-                   const c10::optional<at::Tensor>& bias, at::ScalarType dtype) {
+// a [R, K] (bf16 rows of stride lda) times the decoded weight wd on the tiled GEMM: b_tr = false: a wdᵀ (wd [N, K]),
+// n_out >= N columns (zeros behind N); b_tr = true: a wd (wd [K, N])
+at::Tensor tiled(const at::Tensor& a, int64_t K, const at::Tensor& wd, bool b_tr, int64_t n_out, const float* bias,
+                 at::ScalarType dtype) {
+  auto y = at::empty({a.size(0), n_out}, a.options().dtype(dtype));
+  hyp::GemmTiledArgs g;
+  g.in_dtype = hyp::kBF16;
+  g.out_dtype = dtype_code(dtype);
+  g.A = a.data_ptr();
+  g.B = wd.data_ptr();
+  g.C = y.data_ptr();
+  g.M = (int)a.size(0);
+  g.N = (int)n_out;
+  g.K = (int)K;
+  g.lda = (int)a.size(1);
+  g.ldb = (int)wd.size(1);
+  g.ldc = (int)n_out;
+  g.a_tr = false;
+  g.b_tr = b_tr;
+  g.alpha = 1.f;
+  g.b_rows = b_tr ? (int)n_out : (int)wd.size(0);
+  g.zero = device_zero_page(a.device());
+  if (bias) {
+    g.bias = bias;
+    g.bias_dtype = hyp::kF32;
+  }
+  hyp::mx_gemm_plan(g.M, g.N, g.K, &g.tile, &g.splits);
+  const int sp = hyp::gemm_tiled_splits(g);
+  at::Tensor part;
+  if (sp > 1) {
+    part = at::empty({(int64_t)sp * g.M * g.N}, a.options().dtype(at::kFloat));
+    g.part = part.data_ptr<float>();
+  }
+  HYP_CHECK_HIP(hyp::gemm_tiled(g, cur_stream()));
+  return y;
+}
+
+void check_rows(const at::Tensor& x, const at::Tensor& codes, int64_t n, const char* who) {
   HYP_CHECK_CUDA_TENSOR(x);
-  check_mx(codes, scales, x.size(-1), "mx_rows");
-  const int64_t M = x.size(0), N = codes.size(0), nb = scales.size(1);
-  TORCH_CHECK(x.dim() == 2 && x.scalar_type() == at::kBFloat16 && x.is_contiguous() && x.size(1) == 32 * nb &&
-                  x.device() == codes.device() && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
-                  M <= 65535 * 16 && N < (int64_t)INT32_MAX - 16,
-              "mx_rows: contiguous, 16-byte aligned bf16 x [M, 32 nb] on the weight's device");
-  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "mx_rows: bf16 or fp32 output");
+  TORCH_CHECK(x.dim() == 2 && x.size(1) == n && (x.stride(1) == 1 || n == 1) && x.device() == codes.device() &&
+                  x.size(0) >= 1 && x.size(0) < (1 << 24) && codes.size(0) >= 1 && codes.size(0) < (1 << 24) && n >= 1 && n < (1 << 24),
+              who, ": x [M, ", n, "] with unit column stride on the weight's device, all sizes in [1, 2^24)");
+}
+
+at::Tensor decoded(const at::Tensor& codes, const at::Tensor& scales) {
+  return mx_dequantize(codes, scales, scales.size(1) * 32, at::kBFloat16);
+}
+
+// x [M, K] times the transpose of the 4-bit weight [N, K] (+ fp32 bias) -> [M, N] in x's dtype.
+// tile (A/B): -1 planned, 0 the decoded GEMM, 16 mt + nt the one-launch product
+at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
+                     const c10::optional<at::Tensor>& bias, int64_t tile) {
+  check_mx(codes, scales, x.size(-1), "mx_linear");
+  check_rows(x, codes, x.size(-1), "mx_linear");
   const at::DeviceGuard guard(x.device());
-  auto y = at::empty({M, N}, x.options().dtype(dtype));
-  HYP_CHECK_HIP(hyp::mx_rows(x.data_ptr(), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), (int)M, (int)N, (int)nb,
-                             bias_ptr(bias, N, x.device(), "mx_rows"), dtype_code(dtype), y.data_ptr(), cur_stream()));
-  return y;
+  const int64_t M = x.size(0), N = codes.size(0), nb = scales.size(1), P = pieces_of(x.scalar_type());
+  const float* b = bias_ptr(bias, N, x.device(), "mx_linear");
+  const at::Tensor xp = pieces(x, 32 * nb);
+  const auto dt = P == 1 ? at::kBFloat16 : at::kFloat;
+  int mt, nt;
+  hyp::mx_nt_plan((int)(P * M), (int)N, (int)nb, &mt, &nt);
+  if (tile >= 0) mt = (int)tile / 16, nt = (int)tile % 16;
+  at::Tensor y;
+  if (mt > 0) {
+    y = at::empty({P * M, N}, xp.options().dtype(dt));
+    HYP_CHECK_HIP(hyp::mx_nt(xp.data_ptr(), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), (int)(P * M), (int)N,
+                             (int)nb, P == 1 ? b : nullptr, dtype_code(dt), y.data_ptr(), cur_stream(), mt, nt));
+  } else {
+    const int64_t Np = (N + 7) / 8 * 8;
+    const bool direct = P == 1 && (b == nullptr || Np == N);  // the epilogue's bias has as many elements as columns
+    y = tiled(xp, 32 * nb, decoded(codes, scales), false, Np, direct ? b : nullptr, direct ? at::kBFloat16 : at::kFloat);
+    if (direct) return Np == N ? y : y.narrow(1, 0, N).contiguous();
+  }
+  return P == 1 && mt > 0 ? y : join(y, M, N, b, x.scalar_type());
+}
+
+// dy [M, N] times the 4-bit weight [N, K] -> [M, K] in dy's dtype.  tile (A/B): -1 planned, 0 the decoded GEMM, mt
+at::Tensor mx_linear_dgrad(const at::Tensor& dy, const at::Tensor& codes, const at::Tensor& scales, int64_t K,
+                           int64_t tile) {
+  check_mx(codes, scales, K, "mx_linear_dgrad");
+  check_rows(dy, codes, codes.size(0), "mx_linear_dgrad");
+  TORCH_CHECK(K >= 1 && K < (1 << 24), "mx_linear_dgrad: K in [1, 2^24)");
+  const at::DeviceGuard guard(dy.device());
+  const int64_t M = dy.size(0), N = codes.size(0), nb = scales.size(1), P = pieces_of(dy.scalar_type());
+  const at::Tensor dp = pieces(dy, (N + 7) / 8 * 8);
+  const auto dt = P == 1 ? at::kBFloat16 : at::kFloat;
+  int mt;
+  hyp::mx_nn_plan((int)(P * M), (int)N, (int)nb, &mt);
+  if (tile >= 0) mt = (int)tile;
+  at::Tensor dx;
+  if (mt > 0) {
+    dx = at::empty({P * M, K}, dp.options().dtype(dt));
+    HYP_CHECK_HIP(hyp::mx_nn(dp.data_ptr(), dp.size(1), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), (int)(P * M),
+                             (int)N, (int)nb, (int)K, dtype_code(dt), dx.data_ptr(), cur_stream(), mt));
+  } else {
+    dx = tiled(dp, N, decoded(codes, scales), true, 32 * nb, nullptr, dt);
+    if (P == 1) return 32 * nb == K ? dx : dx.narrow(1, 0, K).contiguous();
+  }
+  return P == 1 ? dx : join(dx, M, K, nullptr, dy.scalar_type());
 }
 
 }  // namespace
@@ -100,11 +177,10 @@ void register_mx_ops(pybind11::module& m) {
   m.def("mx_quantize", &mx_quantize, "rows -> microscaled 4-bit (codes, scales)", pybind11::arg("x"));
   m.def("mx_dequantize", &mx_dequantize, "microscaled 4-bit rows -> values", pybind11::arg("codes"),
         pybind11::arg("scales"), pybind11::arg("cols"), pybind11::arg("dtype"));
-  m.def("mx_pieces", &mx_pieces, "activations as exact bf16 pieces [P R, pitch]", pybind11::arg("x"), pybind11::arg("pitch"));
-  m.def("mx_join", &mx_join, "sum of fp32 piece products (+ bias) in the output dtype", pybind11::arg("part"),
-        pybind11::arg("rows"), pybind11::arg("cols"), pybind11::arg("bias"), pybind11::arg("dtype"));
-  m.def("mx_rows", &mx_rows, "few rows x 4-bit weight (one launch)", pybind11::arg("x"), pybind11::arg("codes"),
-        pybind11::arg("scales"), pybind11::arg("bias"), pybind11::arg("dtype"));
+  m.def("mx_linear", &mx_linear, "x times the transposed 4-bit weight (+ bias)", pybind11::arg("x"), pybind11::arg("codes"),
+        pybind11::arg("scales"), pybind11::arg("bias") = pybind11::none(), pybind11::arg("tile") = -1);
+  m.def("mx_linear_dgrad", &mx_linear_dgrad, "dy times the 4-bit weight", pybind11::arg("dy"), pybind11::arg("codes"),
+        pybind11::arg("scales"), pybind11::arg("K"), pybind11::arg("tile") = -1);
 }
 
 }  // namespace hypbind

@@ -164,78 +164,250 @@ __global__ __launch_bounds__(kQThreads) void mx_join_k(const float* __restrict__
   st1<T>(y + i, s);
 }
 
-// ---- few rows times a 4-bit weight ---------------------------------------------------------------------
-// y [M, N] = x [M, 32 nb] Wt, W [N, 32 nb] in blocks.  A workgroup owns 16 columns of y and 16 MT rows; its
-// 8 waves share the reduction (wave w takes the groups of four blocks w, w + 8, ...), so that the few
-// columns of a thin product still fill the chip and one launch does it: no partial sums in memory.
-// v_mfma_f32_16x16x32_bf16: lane l holds 8 reduction elements of row / column l & 15.  The order of the
-// reduction is free as long as both operands share it: lane group g = l >> 4 takes block 4 kk + g whole, so
-// that a lane's 16-byte load of codes is one block under one scale and feeds four matrix instructions.
-// The eight partial tiles meet in LDS in wave order (the result does not depend on timing).
-constexpr int kRowWaves = 8;
+// ---- activations times a 4-bit weight, decoded on the way to the matrix instructions ---------------------
+// Both products run on v_mfma_f32_16x16x32_bf16 (lane l: 8 reduction elements 8 (l >> 4) .. of row / column
+// l & 15) without LDS or barriers in their loops: the waves of a workgroup share one output tile and
+// split its reduction into contiguous ranges, so that thin products still fill the chip, every wave
+// streams its own operands from L2, and one launch does it.  The partial tiles meet in LDS in wave order
+// (the result does not depend on timing).  Workgroups of one weight tile and different rows are 8 ids
+// apart, on one XCD: the weight comes from HBM once.
+constexpr int kMxWaves = 8;
 
-template <int MT, typename O>
-__global__ __launch_bounds__(kRowWaves * 64) void mx_rows_k(const bf16_t* __restrict__ x, const uint8_t* __restrict__ codes,
-                                                            const uint8_t* __restrict__ scales, int M, int N, int nb,
-                                                            const float* __restrict__ bias, O* __restrict__ y) {
-  __shared__ float part[kRowWaves][MT][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
-  const int64_t K = (int64_t)nb * kMxBlock;
-  const int n = n0 + l15;
-  f32x4 acc[MT];
+struct MxArgs {
+  const bf16_t* x;  // NT: [M, 32 nb]; NN: [M, ld]
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* bias;  // NT: [N] or null
+  void* y;
+  int M, N, nb;  // weight [N, 32 nb]
+  int cols;      // NN: columns of y (K of the weight)
+  int64_t ld;    // NN: row stride of x
+};
+
+// workgroup -> (row block, weight tile)
+__device__ __forceinline__ void mx_tile(int rows, int tiles, int* mb, int* tile) {
+  const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+  *mb = i % rows;
+  *tile = (i / rows) * 8 + xcd;
+}
+
+// Lanes 16 g + l hold words w[0..3] of block g of row l; afterwards word j is word g of block j (a 4 x 4
+// transposition over the lane groups): reduction elements 8 g .. 8 g + 7 of block j, as the matrix
+// instruction wants them, so that the activations are read in rows of 64 bytes.
+__device__ __forceinline__ void mx_group_transpose(u32x4& w) {
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+  const u32x2 c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+  const u32x2 d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  w = u32x4{c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ u16x8 mx_fragment(unsigned w, float s) {
+  union {
+    bf16x2 p[4];
+    u16x8 v;
+  } f;
+  f.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0);
+  f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1);
+  f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2);
+  f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
+  return f.v;
+}
+
+// the four scales of a group of blocks as bytes of a word (127, that is 1, behind the row's end)
+__device__ __forceinline__ unsigned mx_group_scales(const uint8_t* row, int b, int nb) {
+  if (b + 4 <= nb) {
+    typedef unsigned u32a __attribute__((aligned(1)));
+    return *reinterpret_cast<const u32a*>(row + b);
+  }
+  unsigned s = 0x7f7f7f7fu;
+  for (int i = 0; i < 4 && b + i < nb; ++i) s = (s & ~(255u << (8 * i))) | ((unsigned)row[b + i] << (8 * i));
+  return s;
+}
+
+// y [M, N] = x Wt (+ bias): a workgroup owns 16 MT rows and 16 NT columns.  The reduction goes in groups of
+// four blocks (128 elements); a lane's 16-byte load of codes is one block of its column.  Groups are loaded
+// one ahead of the matrix instructions that use them.
+template <int MT, int NT, typename O>
+__global__ __launch_bounds__(kMxWaves * 64) void mx_nt_k(const MxArgs a) {
+  extern __shared__ float part[];  // [waves][MT][NT][256]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+  int mb, tile;
+  mx_tile((a.M + 16 * MT - 1) / (16 * MT), (a.N + 16 * NT - 1) / (16 * NT), &mb, &tile);
+  const int n0 = tile * 16 * NT, m0 = mb * 16 * MT;
+  if (n0 >= a.N) return;  // the last ids of a tile count that is no multiple of 8
+  const int64_t K = (int64_t)a.nb * kMxBlock;
+  const int groups = (a.nb + 3) >> 2;
+  const int kb = (int)((int64_t)wave * groups / kMxWaves), ke = (int)((int64_t)(wave + 1) * groups / kMxWaves);
+  f32x4 acc[MT][NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int groups = (nb + 3) >> 2;
-  for (int kk = wave; kk < groups; kk += kRowWaves) {
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Stage {
+    u32x4 w[NT];
+    unsigned s[NT];
+    u16x8 x[MT][4];
+  };
+  auto load = [&](Stage& t, int kk) {
     const int b = kk * 4 + g;
-    u32x4 w = {0u, 0u, 0u, 0u};
-    unsigned sb = 127;
-    const bool in = b < nb;
-    if (in && n < N) {
-      w = *reinterpret_cast<const u32x4*>(codes + ((int64_t)n * nb + b) * 16);
-      sb = scales[(int64_t)n * nb + b];
-    }
-    const float s = mx_scale(sb);
-    u16x8 a[MT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int m = m0 + i * 16 + l15;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[i][j] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (in && m < M) a[i][j] = *reinterpret_cast<const u16x8*>(x + m * K + (int64_t)b * kMxBlock + j * 8);
+    for (int j = 0; j < NT; ++j) {
+      const int n = n0 + 16 * j + l15;
+      t.w[j] = u32x4{0u, 0u, 0u, 0u};
+      t.s[j] = 0x7f7f7f7fu;
+      if (n < a.N) {
+        if (b < a.nb) t.w[j] = *reinterpret_cast<const u32x4*>(a.codes + ((int64_t)n * a.nb + b) * 16);
+        t.s[j] = mx_group_scales(a.scales + (int64_t)n * a.nb, kk * 4, a.nb);
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      union {
-        bf16x2 p[4];
-        u16x8 v;
-      } f;
-      f.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], s, 0);
-      f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], s, 1);
-      f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], s, 2);
-      f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], s, 3);
+    for (int i = 0; i < MT; ++i) {
+      const int m = m0 + 16 * i + l15;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = mfl::mma16<bf16_t>(a[i][j], f.v, acc[i]);
+      for (int q = 0; q < 4; ++q) {
+        t.x[i][q] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (m < a.M && kk * 4 + q < a.nb)
+          t.x[i][q] = *reinterpret_cast<const u16x8*>(a.x + m * K + (int64_t)(kk * 4 + q) * kMxBlock + g * 8);
+      }
     }
-  }
+  };
+  auto use = [&](Stage& t) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
+    for (int j = 0; j < NT; ++j) {
+      mx_group_transpose(t.w[j]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][i][(4 * g + e) * 16 + l15] = acc[i][e];
+      for (int q = 0; q < 4; ++q) {
+        const u16x8 f = mx_fragment(t.w[j][q], mx_scale((t.s[j] >> (8 * q)) & 255u));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = mfl::mma16<bf16_t>(t.x[i][q], f, acc[i][j]);
+      }
+    }
+  };
+  if (kb < ke) {
+    Stage t[2];
+    load(t[0], kb);
+    int kk = kb;
+    for (; kk + 2 <= ke; kk += 2) {
+      load(t[1], kk + 1);
+      use(t[0]);
+      if (kk + 2 < ke) load(t[0], kk + 2);
+      use(t[1]);
+    }
+    if (kk < ke) use(t[0]);
   }
+  constexpr int kTile = MT * NT * 256;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave * kTile + (16 * i + 4 * g + e) * (16 * NT) + 16 * j + l15] = acc[i][j][e];
   __syncthreads();
-  for (int t = threadIdx.x; t < MT * 256; t += kRowWaves * 64) {
-    const int i = t >> 8, r = (t >> 4) & 15, c = t & 15;
-    const int m = m0 + i * 16 + r;
-    if (m >= M || n0 + c >= N) continue;
+  O* y = static_cast<O*>(a.y);
+  for (int t = threadIdx.x; t < kTile; t += kMxWaves * 64) {
+    const int m = m0 + t / (16 * NT), n = n0 + t % (16 * NT);
+    if (m >= a.M || n >= a.N) continue;
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) sum += part[w][i][t & 255];
-    if (bias) sum += bias[n0 + c];
-    st1<O>(y + (int64_t)m * N + n0 + c, sum);
+    for (int w = 0; w < kMxWaves; ++w) sum += part[w * kTile + t];
+    if (a.bias) sum += a.bias[n];
+    st1<O>(y + (int64_t)m * a.N + n, sum);
+  }
+}
+
+// y [M, cols] = x W, x [M, N]: the reduction runs over the weight's rows.  A workgroup owns 16 MT rows and 128
+// columns, 32 weight rows a step: a lane loads 8 elements (4 bytes) of each of 8 weight rows, decodes them
+// under each row's own scale and transposes the 8 x 8 in registers (v_perm), which gives the fragments of
+// columns 8 (l & 15) + c, c = 0..7: no transposed copy of the weight, and 16 consecutive bytes of y a lane.
+template <int MT, typename O>
+__global__ __launch_bounds__(kMxWaves * 64) void mx_nn_k(const MxArgs a) {
+  extern __shared__ float part[];  // [waves][16 MT][128]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+  int mb, tile;
+  mx_tile((a.M + 16 * MT - 1) / (16 * MT), (a.cols + 127) / 128, &mb, &tile);
+  const int k0 = tile * 128, m0 = mb * 16 * MT;
+  if (k0 >= a.cols) return;
+  const int steps = (a.N + 31) >> 5;
+  const int sb = (int)((int64_t)wave * steps / kMxWaves), se = (int)((int64_t)(wave + 1) * steps / kMxWaves);
+  const int blk = (k0 >> 5) + (l15 >> 2);
+  const bool in = blk < a.nb;
+  const uint8_t* cp = a.codes + (int64_t)blk * 16 + (l15 & 3) * 4;
+  const uint8_t* sp = a.scales + blk;
+  f32x4 acc[MT][8];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Stage {
+    unsigned w[8], s[8];
+    u16x8 x[MT];
+  };
+  auto load = [&](Stage& t, int st) {
+    const int n0 = st * 32 + g * 8;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      t.w[r] = 0u;
+      t.s[r] = 127u;
+      if (in && n0 + r < a.N) {
+        t.w[r] = *reinterpret_cast<const unsigned*>(cp + (int64_t)(n0 + r) * a.nb * 16);
+        t.s[r] = sp[(int64_t)(n0 + r) * a.nb];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = m0 + 16 * i + l15;
+      t.x[i] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (m < a.M && n0 < a.N) t.x[i] = *reinterpret_cast<const u16x8*>(a.x + m * a.ld + n0);
+    }
+  };
+  auto use = [&](const Stage& t) {
+    union {
+      u16x8 v;
+      unsigned w[4];
+    } row[8], f;  // row[r].w[q]: columns 2 q, 2 q + 1 of weight row r
+#pragma unroll
+    for (int r = 0; r < 8; ++r) row[r].v = mx_fragment(t.w[r], mx_scale(t.s[r]));
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h)  // rows 2 h, 2 h + 1 of column c
+        f.w[h] = __builtin_amdgcn_perm(row[2 * h + 1].w[c >> 1], row[2 * h].w[c >> 1], (c & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i][c] = mfl::mma16<bf16_t>(t.x[i], f.v, acc[i][c]);
+    }
+  };
+  if (sb < se) {
+    Stage t[2];
+    load(t[0], sb);
+    int st = sb;
+    for (; st + 2 <= se; st += 2) {
+      load(t[1], st + 1);
+      use(t[0]);
+      if (st + 2 < se) load(t[0], st + 2);
+      use(t[1]);
+    }
+    if (st < se) use(t[0]);
+  }
+  constexpr int kTile = MT * 16 * 128;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float* p = part + wave * kTile + (16 * i + 4 * g + e) * 128 + 8 * l15;
+      reinterpret_cast<float4*>(p)[0] = make_float4(acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(acc[i][4][e], acc[i][5][e], acc[i][6][e], acc[i][7][e]);
+    }
+  __syncthreads();
+  O* y = static_cast<O*>(a.y);
+  for (int t = threadIdx.x; t < kTile; t += kMxWaves * 64) {
+    const int m = m0 + (t >> 7), k = k0 + (t & 127);
+    if (m >= a.M || k >= a.cols) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMxWaves; ++w) sum += part[w * kTile + t];
+    st1<O>(y + (int64_t)m * a.cols + k, sum);
   }
 }
 
@@ -298,24 +470,103 @@ hipError_t mx_join(int dtype, const float* part, int pieces, int64_t rows, int c
   return hipGetLastError();
 }
 
-hipError_t mx_rows(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
-                   int out_dtype, void* y, hipStream_t stream) {
+namespace {
+
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+template <typename K>
+hipError_t mx_launch(K kernel, int rows, int tiles, size_t lds, const MxArgs& a, hipStream_t stream) {
+  const int64_t grid = (int64_t)rows * ((tiles + 7) / 8 * 8);
+  if (grid >= kMxGridMax) return hipErrorInvalidValue;
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kMxWaves * 64), lds, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Measured (MI355X, bf16): the one-launch product against decoding the weight (8 us for 4096 x 4096, 18 for 11008 x
+// 4096) plus the tiled GEMM (17 us at least): the larger tiles while they give every CU a workgroup.
+void mx_nt_plan(int M, int N, int nb, int* mt, int* nt) {
+  struct T {
+    int mt, nt;
+  };
+  static const T kOrder[] = {{4, 4}, {2, 4}, {2, 2}, {1, 2}, {1, 1}};
+  const int64_t work = (int64_t)M * N * nb;
+  *mt = *nt = 0;
+  if (M > 128 && work > (int64_t)256 * 4096 * 128) return;
+  for (const T& t : kOrder) {
+    *mt = t.mt;
+    *nt = t.nt;
+    if (16 * t.mt <= M && (int64_t)ceil_div(M, 16 * t.mt) * ceil_div(N, 16 * t.nt) >= 256) return;
+  }
+}
+
+void mx_nn_plan(int M, int N, int nb, int* mt) {
+  const int64_t work = (int64_t)M * N * nb;
+  *mt = M > 128 && work > (int64_t)256 * 4096 * 128 ? 0 : (ceil_div(M, 32) * ceil_div(nb, 4) >= 256 ? 2 : 1);
+}
+
+// The tiled GEMM's 256x256 ping-pong tile (one workgroup a CU) or its 128x128 tile (two a CU), by the rounds that
+// their workgroups need: a 32-deep step of a round takes 1.0 us / 0.62 us (measured at 2032 .. 4064 rows), a split
+// another pass over fp32 partial sums.
+void mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
+  double best = 1e30;
+  *tile = 3;
+  *splits = 1;
+  for (int t : {8, 3}) {
+    const int b = t == 8 ? 256 : 128;
+    if (t == 8 && (M < 256 || N < 256)) continue;
+    const int64_t tiles = (int64_t)ceil_div(M, b) * ceil_div(N, b);
+    for (int s : {1, 2, 4, 8}) {
+      if (s > 1 && K / s < 512) break;
+      const int slots = t == 8 ? 256 : 512;
+      double us = (double)((tiles * s + slots - 1) / slots) * ceil_div(ceil_div(K, 32), s) * (t == 8 ? 1.0 : 0.62);
+      if (s > 1) us += 4.0 + (double)M * N * 4.0 * (s + 1) / 4e6;
+      if (us < best) {
+        best = us;
+        *tile = t;
+        *splits = s;
+      }
+    }
+  }
+}
+
+hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
+                 int out_dtype, void* y, hipStream_t stream, int mt, int nt) {
   if (M == 0 || N == 0) return hipSuccess;
   if (out_dtype != kBF16 && out_dtype != kF32) return hipErrorInvalidValue;
-  const int mt = M <= 16 ? 1 : (M <= 32 ? 2 : 4);
-  const dim3 grid((N + 15) / 16, (M + 16 * mt - 1) / (16 * mt)), block(kRowWaves * 64);
-  if (grid.y > 65535) return hipErrorInvalidValue;
-  const bf16_t* xp = static_cast<const bf16_t*>(x);
-#define HYP_MX_ROWS(MT)                                                                                       \
-  if (out_dtype == kBF16)                                                                                     \
-    hipLaunchKernelGGL((mx_rows_k<MT, bf16_t>), grid, block, 0, stream, xp, codes, scales, M, N, nb, bias,    \
-                       static_cast<bf16_t*>(y));                                                              \
-  else                                                                                                        \
-    hipLaunchKernelGGL((mx_rows_k<MT, float>), grid, block, 0, stream, xp, codes, scales, M, N, nb, bias,     \
-                       static_cast<float*>(y));
-  if (mt == 1) { HYP_MX_ROWS(1) } else if (mt == 2) { HYP_MX_ROWS(2) } else { HYP_MX_ROWS(4) }
-#undef HYP_MX_ROWS
-  return hipGetLastError();
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, bias, y, M, N, nb, 0, 0};
+#define HYP_MX_NT(MT, NT)                                                                                      \
+  if (mt == MT && nt == NT) {                                                                                  \
+    const size_t lds = sizeof(float) * kMxWaves * MT * NT * 256;                                               \
+    const int rows = ceil_div(M, 16 * MT), tiles = ceil_div(N, 16 * NT);                                       \
+    return out_dtype == kBF16 ? mx_launch(mx_nt_k<MT, NT, bf16_t>, rows, tiles, lds, a, stream)                \
+                              : mx_launch(mx_nt_k<MT, NT, float>, rows, tiles, lds, a, stream);                \
+  }
+  HYP_MX_NT(1, 1) HYP_MX_NT(1, 2) HYP_MX_NT(2, 2) HYP_MX_NT(2, 4) HYP_MX_NT(4, 4)
+#undef HYP_MX_NT
+  return hipErrorInvalidValue;
+}
+
+hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, int cols,
+                 int out_dtype, void* y, hipStream_t stream, int mt) {
+  if (M == 0 || cols == 0) return hipSuccess;
+  if ((out_dtype != kBF16 && out_dtype != kF32) || ld % 8 != 0) return hipErrorInvalidValue;
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld};
+#define HYP_MX_NN(MT)                                                                                          \
+  if (mt == MT) {                                                                                              \
+    const size_t lds = sizeof(float) * kMxWaves * MT * 2048;                                                   \
+    const int rows = ceil_div(M, 16 * MT), tiles = ceil_div(cols, 128);                                        \
+    return out_dtype == kBF16 ? mx_launch(mx_nn_k<MT, bf16_t>, rows, tiles, lds, a, stream)                    \
+                              : mx_launch(mx_nn_k<MT, float>, rows, tiles, lds, a, stream);                    \
+  }
+  HYP_MX_NN(1) HYP_MX_NN(2)
+#undef HYP_MX_NN
+  return hipErrorInvalidValue;
 }
 
 }  // namespace hyp

@@ -13,8 +13,8 @@ is one of 0, .5, 1, 1.5, 2, 3, 4, 6 with a sign (e2m1), two to a byte, the first
   activations are split into two or three bf16 numbers whose sum they are, and lose nothing either.
   The weight is frozen: it has no gradient.
 
-Few rows (``ROWS_MAX``) run on one launch that reads the codes straight into the matrix instructions;
-more rows decode the weight to bf16 once (a buffer of the call) and run on the tiled GEMM.
+Products up to a few hundred rows run on one launch that decodes the codes on their way to the matrix
+instructions; larger ones decode the weight to bf16 once (a buffer of the call) and run on the tiled GEMM.
 """
 from __future__ import annotations
 
@@ -31,7 +31,6 @@ from .linear import bias_grad
 
 BLOCK = 32
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-ROWS_MAX = 64  # rows (times bf16 pieces) of the one-launch product
 
 
 class MXFP4Tensor:
@@ -123,86 +122,51 @@ def quantize_mxfp4(x: torch.Tensor) -> MXFP4Tensor:
     return MXFP4Tensor(codes, scales, tuple(x.shape))
 
 
-_PIECES = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
+def _unit_rows(x: torch.Tensor, n: int) -> torch.Tensor:
+    """[M, n] with unit column stride (a view where it is one)."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, n)
+    return x2 if n <= 1 or x2.stride(1) == 1 else x2.contiguous()
 
 
-def _bf16_rows(x2: torch.Tensor, pitch: int) -> torch.Tensor:
-    """x2 [M, n] as bf16 pieces [P M, pitch] whose sum it is, zeros behind n (x2 itself where it is that)."""
-    if x2.shape[1] > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    if x2.dtype == torch.bfloat16 and x2.shape[1] == pitch and x2.is_contiguous() and x2.data_ptr() % 16 == 0:
-        return x2
-    return _native.native().mx_pieces(x2, pitch)
-
-
-def _fwd(x2: torch.Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
-    """x2 [M, K] Wᵀ (+ bias) in x2's dtype."""
-    C = _native.native()
-    M, N, Kp = x2.shape[0], w.shape[0], w.scales.shape[1] * BLOCK
-    xp = _bf16_rows(x2, Kp)
-    P = _PIECES[x2.dtype]
-    b32 = None if bias is None else bias.detach().float().contiguous()
-    if P * M <= ROWS_MAX:
-        _native.count("mxfp4_rows")
-        if P == 1:
-            return C.mx_rows(xp, w.codes, w.scales, b32, torch.bfloat16)
-        return C.mx_join(C.mx_rows(xp, w.codes, w.scales, None, torch.float32), M, N, b32, x2.dtype)
-    _native.count("mxfp4_gemm")
-    wd = w._rows(torch.bfloat16, Kp)
-    Np = -(-N // 8) * 8
-    if P == 1 and (bias is None or Np == N):
-        if b32 is not None and b32.data_ptr() % 16:
-            b32 = b32.clone()
-        y = C.gemm(xp, wd, bias=b32, n_out=Np if Np > N else -1)
-        return y if Np == N else y[:, :N].contiguous()
-    return C.mx_join(C.gemm(xp, wd, out_dtype=torch.float32, n_out=Np if Np > N else -1), M, N, b32, x2.dtype)
-
-
-def _dgrad(dy2: torch.Tensor, w: MXFP4Tensor) -> torch.Tensor:
-    """dy2 [M, N] W in dy2's dtype."""
-    C = _native.native()
-    M, N, K = dy2.shape[0], w.shape[0], w.shape[1]
-    Kp = w.scales.shape[1] * BLOCK
-    dp = _bf16_rows(dy2, -(-N // 8) * 8)
-    _native.count("mxfp4_dgrad_gemm")
-    wd = w._rows(torch.bfloat16, Kp)
-    if _PIECES[dy2.dtype] == 1:
-        dx = C.gemm(dp[:, :N], wd, b_tr=True)
-        return dx if Kp == K else dx[:, :K].contiguous()
-    return C.mx_join(C.gemm(dp[:, :N], wd, b_tr=True, out_dtype=torch.float32), M, K, None, dy2.dtype)
+def _bias32(bias: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if bias is None:
+        return None
+    b = bias.detach().float().contiguous()
+    return b if b.data_ptr() % 16 == 0 else b.clone()
 
 
 class _MXLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, w):
-        x2 = x.reshape(-1, x.shape[-1])
-        native = _native.use_native(x2, w.codes, op="mxfp4")
-        if x2.shape[0] == 0 or w.shape[0] == 0 or w.shape[1] == 0:
-            y = x2.new_zeros(x2.shape[0], w.shape[0]) + (0 if bias is None else bias.to(x2.dtype))
+        N, K = w.shape
+        native = _native.use_native(x, w.codes, op="mxfp4")
+        if x.numel() == 0 or N == 0:
+            y = x.new_zeros(*x.shape[:-1], N) + (0 if bias is None else bias.to(x.dtype))
         elif native:
-            y = _fwd(x2, w, bias)
+            _native.count("mxfp4_linear")
+            y = _native.native().mx_linear(_unit_rows(x, K), w.codes, w.scales, _bias32(bias))
         else:
-            y = x2.float() @ w._rows(torch.float32, w.shape[1]).t()
+            y = x.float() @ w._rows(torch.float32, K).t()
             y = (y if bias is None else y + bias.float()).to(x.dtype)
         ctx.w, ctx.native, ctx.xshape, ctx.bdtype = w, native, x.shape, None if bias is None else bias.dtype
-        return y.view(*x.shape[:-1], w.shape[0])
+        return y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         w = ctx.w
-        dy2 = dy.reshape(-1, w.shape[0])
+        N, K = w.shape
         dx = db = None
         if ctx.needs_input_grad[0]:
-            if dy2.shape[0] == 0 or w.shape[0] == 0 or w.shape[1] == 0:
-                dx = dy2.new_zeros(dy2.shape[0], w.shape[1])
+            if dy.numel() == 0 or K == 0:
+                dx = dy.new_zeros(ctx.xshape)
             elif ctx.native:
-                dx = _dgrad(dy2, w)
+                _native.count("mxfp4_dgrad")
+                dx = _native.native().mx_linear_dgrad(_unit_rows(dy, N), w.codes, w.scales, K).view(ctx.xshape)
             else:
-                dx = (dy2.float() @ w._rows(torch.float32, w.shape[1])).to(dy2.dtype)
-            dx = dx.view(ctx.xshape)
+                dx = (dy.float() @ w._rows(torch.float32, K)).to(dy.dtype)
         if ctx.bdtype is not None and ctx.needs_input_grad[1]:
-            db = bias_grad(dy2.contiguous(), ctx.bdtype)
+            db = bias_grad(dy.reshape(-1, N).contiguous(), ctx.bdtype)
         return dx, db, None
 
 

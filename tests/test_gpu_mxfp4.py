@@ -85,11 +85,30 @@ def test_strided_activations(M):
     check_linear(96, 40, M, torch.bfloat16, False, view=lambda t: t.t().contiguous().t())
 
 
-def test_both_sides_of_the_row_limit_agree_in_dtype_and_shape():
-    for M in (64, 65):
-        w, x, dy, y, dx = check_linear(M, 64, 96, torch.bfloat16, False)
-        y3 = mxfp4_linear(x.view(1, M, 96), w)
-        assert torch.equal(y3[0], y)  # deterministic, and batch dimensions are rows
+@pytest.mark.parametrize("M,N,K", [(1, 100, 160), (33, 300, 96), (70, 72, 384), (200, 264, 1056)])
+def test_every_tile_gives_the_same_product(M, N, K):
+    C = _native.native()
+    g = torch.Generator().manual_seed(M)
+    w = quantize_mxfp4(torch.randn(N, K, generator=g).to(DEV))
+    W = decoded(w.codes, w.scales, K).to(DEV)
+    b = torch.randn(N, generator=g).to(DEV)
+    for dtype in (torch.bfloat16, torch.float32):
+        x, dy = torch.randn(M, K, generator=g).to(dtype).to(DEV), torch.randn(M, N, generator=g).to(dtype).to(DEV)
+        xd, dd = x.double(), dy.double()
+        want = xd @ W.t() + b.double()
+        bound = product_bound(xd, W.t(), dtype) + (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * (b.double().abs() + want.abs())
+        for mt, nt in ((0, 0), (1, 1), (1, 2), (2, 2), (2, 4), (4, 4)):
+            y = C.mx_linear(x, w.codes, w.scales, b, 16 * mt + nt)
+            assert ((y.double() - want).abs() <= bound).all(), (mt, nt)
+        for mt in (0, 1, 2):
+            dx = C.mx_linear_dgrad(dy, w.codes, w.scales, K, mt)
+            assert ((dx.double() - dd @ W).abs() <= product_bound(dd, W, dtype)).all(), mt
+
+
+def test_batches_are_rows():
+    w, x, dy, y, dx = check_linear(65, 64, 96, torch.bfloat16, False)
+    assert torch.equal(mxfp4_linear(x.view(1, 65, 96), w)[0], y)
+    assert torch.equal(mxfp4_linear(x[3], w), mxfp4_linear(x[3:4], w)[0])
 
 
 def test_non_finite_activations_and_weights():
@@ -149,7 +168,6 @@ def test_other_stream_and_graph_replays(M):
 def test_kernels_are_reached():
     w = quantize_mxfp4(torch.randn(64, 64, device=DEV))
     _native.reset_counters()
-    for M, name in ((4, "mxfp4_rows"), (80, "mxfp4_gemm")):
-        x = torch.randn(M, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
-        mxfp4_linear(x, w).sum().backward()
-        assert _native.counters().get(name) == 1
+    x = torch.randn(4, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    mxfp4_linear(x, w).sum().backward()
+    assert _native.counters() == {"mxfp4_linear": 1, "mxfp4_dgrad": 1}
