@@ -92,6 +92,8 @@ def _common_flags(inc, abi, debug: bool = False) -> List[str]:
         "-fPIC",
         f"--offload-arch={ARCH}",
         "-munsafe-fp-atomics",
+        # no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results now and then
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-Wno-unused-result",
         "-Wno-deprecated-declarations",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(abi)}",
