@@ -60,16 +60,20 @@ LogitRows logit_rows(const at::Tensor& z, const at::Tensor& target, const char* 
   return r;
 }
 
-// (logprobs, entropy, stats [rows, 3], top logprobs [rows, k], top ids [rows, k])
+// (logprobs [...], entropy [...], stats [rows, 3], top logprobs [..., k], top ids [..., k])
 std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& z, const at::Tensor& target, int64_t k, int64_t ignore_index,
                                            double inv_t) {
   const LogitRows r = logit_rows(z, target, "token_logprobs_fwd");
   TORCH_CHECK(k >= 0 && k <= hyp::kTokenTopMax && k <= r.V, "token_logprobs_fwd: k must be in [0, min(V, ",
               hyp::kTokenTopMax, ")]");
+  TORCH_CHECK(k == 0 || r.V <= hyp::kTokenTopVocab, "token_logprobs_fwd: alternatives for at most ", hyp::kTokenTopVocab, " tokens");
   const at::DeviceGuard guard(z.device());
   auto fopt = z.options().dtype(at::kFloat);
-  auto lp = at::empty({r.rows}, fopt), ent = at::empty({r.rows}, fopt), stats = at::empty({r.rows, 3}, fopt);
-  auto tl = at::empty({r.rows, k}, fopt), ti = at::empty({r.rows, k}, z.options().dtype(at::kLong));
+  const auto lead = z.sizes().slice(0, z.dim() - 1);
+  auto topk = lead.vec();
+  topk.push_back(k);
+  auto lp = at::empty(lead, fopt), ent = at::empty(lead, fopt), stats = at::empty({r.rows, 3}, fopt);
+  auto tl = at::empty(topk, fopt), ti = at::empty(topk, z.options().dtype(at::kLong));
   HYP_CHECK_HIP(hyp::token_logprobs_fwd(dtype_code(z), z.data_ptr(), r.s0, r.s1, r.inner, r.rows, r.V,
                                         target.data_ptr<int64_t>(), ignore_index, (float)inv_t, lp.data_ptr<float>(),
                                         ent.data_ptr<float>(), stats.data_ptr<float>(), (int)k, tl.data_ptr<float>(),

@@ -144,6 +144,7 @@ namespace hyp {
 // contiguous [rows, V].  A launch holds fewer than kTokenRowsMax workgroups of 256 threads.
 constexpr int kTokenTopMax = 32;
 constexpr int64_t kTokenRowsMax = int64_t(1) << 24;
+constexpr int kTokenTopVocab = 1 << 18;  // with alternatives: V / 8 bytes of LDS
 hipError_t token_logprobs_fwd(int dtype, const void* z, int64_t s0, int64_t s1, int inner, int64_t rows, int V,
                               const int64_t* target, int64_t ignore, float inv_t, float* logp, float* ent, float* stats,
                               int k, float* top_lp, int64_t* top_id, hipStream_t stream);

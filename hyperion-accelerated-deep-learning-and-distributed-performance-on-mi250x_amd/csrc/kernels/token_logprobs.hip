@@ -9,14 +9,20 @@
 // and from the saved (m, log2 s, H), with q_j = t_j - log2 s, p_j = 2^q_j:
 //   dz_j = [ dlogp (delta_j - p_j) - dH p_j (q_j ln 2 + H) ] / T
 // Sums are fp32.  The forward reads every logit once, the backward reads it once and writes its
-// gradient once: HBM bounds both (about 10 VALU slots per logit, of which exp2 takes 4).
+// gradient once: HBM bounds both, with about 11 VALU slots per logit (exp2 takes 4 of them) close behind.
+// Measured, bf16: 2032 x 50257 forward 38 us (5.4 TB/s); 4064 x 50257 forward 105 us and backward 139 us, together
+// 5.0 TB/s, a large copy's rate (reading the first rows past the last-level cache, or the rows backwards in the
+// backward, changed nothing); one row with 20 alternatives 12 us, of which the launch is 3.
 //
-// Rows start at any element (V = 50257 rows of 2-byte logits are 2-byte aligned): 16-byte loads and
-// stores at the row's own alignment, which gfx950 global memory takes, instead of a scalar head.
+// Rows start at any element (V = 50257 rows of 2-byte logits are 2-byte aligned).  The forward reads the
+// 16-byte aligned part of a row in 16-byte pieces; the backward, whose logits and gradient rows need not
+// have the same alignment, loads and stores 16 bytes at the row's own.
 //
 // An empty row (every logit -inf) has logprob -inf, entropy 0 and no gradient; a NaN or +inf logit
 // makes its row's results and gradient NaN; a target outside [0, V) is never read and makes the
 // row's logprob and gradient NaN; a row whose target is ignore_index is not read: 0 everywhere, ids -1.
+#include <type_traits>
+
 #include "hyp_common.h"
 #include "hyp_kernels.h"
 
@@ -25,23 +31,25 @@ namespace {
 
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kFloor = -200.f;  // 2^-200 is 0 in fp32: a finite stand-in for -inf in products with p = 0
-constexpr int kTopCap = 1024;     // candidates of the top alternatives kept in LDS
+constexpr int kTopCap = 1024;     // candidates of the top alternatives kept in LDS, and batches that hold them
+constexpr int kTopPrefix = 1024;  // ids looked at for logits equal to the bound
 
-typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at a row's own alignment
 
 template <typename T>
-struct Row16 {  // 16 bytes of a row, at the row's alignment
+struct Row16 {  // 16 bytes of a row
   static constexpr int N = 16 / (int)sizeof(T);
-  static __device__ __forceinline__ u32x4a raw(const T* p) { return *reinterpret_cast<const u32x4a*>(p); }
-  static __device__ __forceinline__ void open(const u32x4a& r, float (&v)[N]);
+  static __device__ __forceinline__ u32x4 raw(const T* p) { return *reinterpret_cast<const u32x4a*>(p); }
+  static __device__ __forceinline__ void open(const u32x4& r, float (&v)[N]);
 };
 template <>
-__device__ __forceinline__ void Row16<float>::open(const u32x4a& r, float (&v)[4]) {
+__device__ __forceinline__ void Row16<float>::open(const u32x4& r, float (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
 }
 template <>
-__device__ __forceinline__ void Row16<bf16_t>::open(const u32x4a& r, float (&v)[8]) {
+__device__ __forceinline__ void Row16<bf16_t>::open(const u32x4& r, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[2 * i] = __uint_as_float(r[i] << 16);
@@ -49,7 +57,7 @@ __device__ __forceinline__ void Row16<bf16_t>::open(const u32x4a& r, float (&v)[
   }
 }
 template <>
-__device__ __forceinline__ void Row16<f16_t>::open(const u32x4a& r, float (&v)[8]) {
+__device__ __forceinline__ void Row16<f16_t>::open(const u32x4& r, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[2 * i] = f16_lo(r[i]);
@@ -80,17 +88,18 @@ __device__ __forceinline__ Run run_join(const Run& a, const Run& b, float c) {
   return {m, a.s * fa + b.s * fb, fa * (a.u + fmaxf(da, kFloor) * a.s) + fb * (b.u + fmaxf(db, kFloor) * b.s)};
 }
 
-template <int N>
-__device__ __forceinline__ void run_add(Run& r, const float (&v)[N], float c) {
-  float m = r.m;
-#pragma unroll
-  for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
-  if (m > r.m) {  // also the first values: from m = -inf the old sums are 0
-    const float d = (r.m - m) * c, f = exp2f(d);
+// takes `mx`, the largest of the logits to be added next, into the running maximum
+__device__ __forceinline__ void run_raise(Run& r, float mx, float c) {
+  if (mx > r.m) {  // also the first values: from m = -inf the old sums are 0
+    const float d = (r.m - mx) * c, f = exp2f(d);
     r.u = f * (r.u + fmaxf(d, kFloor) * r.s);
     r.s *= f;
-    r.m = m;
+    r.m = mx;
   }
+}
+// adds N logits that are not above the running maximum
+template <int N>
+__device__ __forceinline__ void run_add(Run& r, const float (&v)[N], float c) {
   const float at = r.m == -INFINITY ? 0.f : r.m;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -98,6 +107,13 @@ __device__ __forceinline__ void run_add(Run& r, const float (&v)[N], float c) {
     r.s += e;
     r.u = fmaf(e, fmaxf(t, kFloor), r.u);
   }
+}
+template <int N>
+__device__ __forceinline__ float largest(const float (&v)[N]) {
+  float mx = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mx = fmaxf(mx, v[i]);
+  return mx;
 }
 
 // order of the alternatives: larger logit first (NaN above everything, -0 = +0), then the lower id
@@ -134,20 +150,42 @@ __device__ __forceinline__ const T* row_ptr(const LpArgs& a, int64_t r) {
   return static_cast<const T*>(a.z) + (r / a.inner) * a.s0 + (r % a.inner) * a.s1;
 }
 
-// One workgroup per row.  TOP: also the k most likely tokens.
-//   1. every thread keeps the key of its largest logit during the pass; the r-th largest of each
-//      full wave, r = ceil(k / full waves), bounds the k-th largest of the row from below (their
-//      smallest is passed by at least k logits);
-//   2. a second sweep (cache) collects the keys that reach the bound into LDS, about 2k..6k of them,
-//      and every candidate writes itself to the place given by how many are larger.
-//   Were there more candidates than fit (orders made to do so), k sweeps pick one maximum each.
-template <typename T, int THREADS, bool TOP>
+// the r-th largest of the 64 lanes' values (with repetitions), in every lane
+__device__ __forceinline__ float wave_rth(float v, int r) {
+  const int lane = threadIdx.x & 63;
+  bool in = true;
+  float top = 0.f;
+  for (int i = 0; i < r; ++i) {
+    top = wave_max(in ? v : -INFINITY);
+    const uint64_t who = __ballot(in && v == top);
+    if (who != 0 && lane == __ffsll((unsigned long long)who) - 1) in = false;
+  }
+  return top;
+}
+
+// One workgroup per row: up to 15 elements before the first and behind the last 16-byte boundary, one to a
+// thread, and the aligned body in batches of U loads a thread (a long read reaches 6.2 TB/s aligned, 5.2
+// at odd elements).
+// TOP: also the k most likely tokens.
+//   1. during the pass every batch's largest logit goes to LDS; with r = ceil(k / full waves), T is the
+//      smallest of the full waves' r-th largest thread maxima: at least k logits are >= T;
+//   2. the batches that hold more than T (their maxima say which, nothing is read again for it) are read
+//      again, a few dozen, and their logits above T become candidates;
+//   3. if these are fewer than k, logits equal to T follow in the order of their ids: a mask's value,
+//      which the first 1024 ids hold often enough;
+//   4. every candidate writes itself to the place given by how many are larger.
+//   Where that does not serve (a NaN or +inf in the row, more candidates than fit, ties elsewhere), k sweeps
+//   over the row pick one maximum each.
+template <typename T, int THREADS, int U, bool TOP>
 __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
-  constexpr int N = Row16<T>::N, W = THREADS / 64, U = 4;
+  constexpr int N = Row16<T>::N, W = THREADS / 64;
+  extern __shared__ float batch_max[];  // TOP: [iterations][THREADS]
   __shared__ Run wr[W];
   __shared__ uint64_t cand[TOP ? kTopCap : 1];
-  __shared__ uint64_t wkey[W];
-  __shared__ int ncand;
+  __shared__ int batches[TOP ? kTopCap : 1];
+  __shared__ uint64_t wkey[TOP ? W : 1];
+  __shared__ float wtop[TOP ? W : 1];
+  __shared__ int nbatch, ncand;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t tgt = a.target[row];
@@ -164,37 +202,52 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
     return;
   }
   const T* z = row_ptr<T>(a, row);
-  const int nv = a.V / N, tail = nv * N;
+  const int head = min(a.V, (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T));
+  const int nv = (a.V - head) / N, tail = head + nv * N;  // 16-byte pieces; elements [0, head) and [tail, V) are single
+  const u32x4* body = reinterpret_cast<const u32x4*>(z + head);
+  const int one = tid < head ? tid : tid - head + tail;   // this thread's single element, if any
+  const bool has_one = one < a.V && tid < head + a.V - tail;
+  const float lone = has_one ? ld1<T>(z + one) : -INFINITY;
   Run run{-INFINITY, 0.f, 0.f};
-  uint64_t best = 0;
-  auto take = [&](const u32x4a& raw, int v) {
-    float x[N];
-    Row16<T>::open(raw, x);
-    run_add<N>(run, x, a.c);
-    if (TOP) {
+  float best = -INFINITY;
+  int it = 0;
+  auto batch = [&](int v0, auto whole) {  // pieces v0, v0 + THREADS, ...; whole: all U of them exist
+    u32x4 r[U];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint64_t k = top_key(x[i], v * N + i);
-        best = k > best ? k : best;
-      }
+    for (int i = 0; i < U; ++i) {
+      r[i] = u32x4{0u, 0u, 0u, 0u};
+      if (whole || v0 + i * THREADS < nv)
+        r[i] = body[v0 + i * THREADS];
     }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (!whole && v0 + i * THREADS >= nv) break;
+      float x[N];
+      Row16<T>::open(r[i], x);
+      top = fmaxf(top, largest<N>(x));
+    }
+    run_raise(run, top, a.c);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (!whole && v0 + i * THREADS >= nv) break;
+      float x[N];
+      Row16<T>::open(r[i], x);
+      run_add<N>(run, x, a.c);
+    }
+    if (TOP) {
+      batch_max[it * THREADS + tid] = top;
+      best = fmaxf(best, top);
+    }
+    ++it;
   };
-  int v = tid;
-  for (; v + (U - 1) * THREADS < nv; v += U * THREADS) {
-    u32x4a r[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) r[i] = Row16<T>::raw(z + (int64_t)(v + i * THREADS) * N);
-#pragma unroll
-    for (int i = 0; i < U; ++i) take(r[i], v + i * THREADS);
-  }
-  for (; v < nv; v += THREADS) take(Row16<T>::raw(z + (int64_t)v * N), v);
-  if (tail + tid < a.V) {
-    const float x[1] = {ld1<T>(z + tail + tid)};
+  const int whole_end = nv / (U * THREADS) * (U * THREADS);
+  for (int v0 = tid; v0 < whole_end; v0 += U * THREADS) batch(v0, std::true_type{});
+  if (whole_end + tid < nv) batch(whole_end + tid, std::false_type{});
+  if (has_one) {
+    const float x[1] = {lone};
+    run_raise(run, lone, a.c);
     run_add<1>(run, x, a.c);
-    if (TOP) {
-      const uint64_t k = top_key(x[0], tail + tid);
-      best = k > best ? k : best;
-    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1)
@@ -202,17 +255,12 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
   if (lane == 0) wr[wv] = run;
   int full = 0;
   if (TOP) {
-    full = min(W, nv / 64);  // waves whose every thread holds a logit
+    full = min(W, nv / 64);  // waves whose every thread holds a piece
     if (wv < full) {
-      const int rounds = (a.k + full - 1) / full;
-      uint64_t mine = best, top = 0;
-      for (int i = 0; i < rounds; ++i) {
-        top = shfl_max64(mine);
-        if (mine == top) mine = 0;  // keys differ in their ids
-      }
-      if (lane == 0) wkey[wv] = top;
+      const float t = wave_rth(best, (a.k + full - 1) / full);
+      if (lane == 0) wtop[wv] = t;
     }
-    if (tid == 0) ncand = 0;
+    if (tid == 0) nbatch = ncand = 0;
   }
   __syncthreads();
   run = lane < W ? wr[lane] : Run{-INFINITY, 0.f, 0.f};
@@ -234,33 +282,57 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
     a.stats[3 * row + 2] = h;
   }
   if (!TOP) return;
-  uint64_t bound = full > 0 ? wkey[0] : 0;
-  for (int i = 1; i < full; ++i) bound = wkey[i] < bound ? wkey[i] : bound;
-  auto put = [&](float x, int id) {
-    const uint64_t k = top_key(x, id);
-    if (k >= bound) {
-      const int at = atomicAdd(&ncand, 1);
-      if (at < kTopCap) cand[at] = k;
-    }
-  };
-  for (v = tid; v < nv; v += THREADS) {
-    float x[N];
-    Row16<T>::open(Row16<T>::raw(z + (int64_t)v * N), x);
-#pragma unroll
-    for (int i = 0; i < N; ++i) put(x[i], v * N + i);
-  }
-  if (tail + tid < a.V) put(ld1<T>(z + tail + tid), tail + tid);
-  __syncthreads();
-  const int n = ncand;
   auto write = [&](int at, uint64_t key) {
     const int id = (int)(0xffffffffu - (uint32_t)key);
     a.top_id[row * a.k + at] = id;
     a.top_lp[row * a.k + at] = empty ? -INFINITY : fmaf(ld1<T>(z + id) - m, a.inv_t, -ls * kLn2);
   };
-  if (n <= kTopCap) {
+  auto put = [&](float x, int id) {
+    const int at = atomicAdd(&ncand, 1);
+    if (at < kTopCap) cand[at] = top_key(x, id);
+  };
+  bool served = run.s == run.s;  // uniform, like every decision below
+  if (served && full == 0) {  // a short row: every logit is a candidate
+    for (int i = tid; i < a.V; i += THREADS) put(ld1<T>(z + i), i);
+  } else if (served) {
+    float bound = wtop[0];
+    for (int i = 1; i < full; ++i) bound = fminf(bound, wtop[i]);
+    for (int i = 0; i < it; ++i)
+      if (batch_max[i * THREADS + tid] > bound) {
+        const int at = atomicAdd(&nbatch, 1);
+        if (at < kTopCap) batches[at] = i * THREADS + tid;
+      }
+    if (has_one && lone > bound) put(lone, one);
+    __syncthreads();
+    const int nb = nbatch;
+    served = nb <= kTopCap;
+    if (served) {
+      for (int i = tid; i < nb * U; i += THREADS) {
+        const int b = batches[i / U], v = (b / THREADS) * (U * THREADS) + (i % U) * THREADS + b % THREADS;
+        if (v >= nv) continue;
+        float x[N];
+        Row16<T>::open(body[v], x);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (x[j] > bound) put(x[j], head + v * N + j);
+      }
+      __syncthreads();
+      const bool few = ncand < a.k;
+      __syncthreads();
+      if (few)
+        for (int i = tid; i < min(a.V, kTopPrefix); i += THREADS) {
+          const float x = ld1<T>(z + i);
+          if (x == bound) put(x, i);
+        }
+    }
+  }
+  __syncthreads();
+  const int n = ncand;
+  if (served && n >= a.k && n <= kTopCap) {
     for (int i = tid; i < n; i += THREADS) {
       const uint64_t key = cand[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += cand[j] > key;
       if (rank < a.k) write(rank, key);
     }
@@ -268,21 +340,14 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
   }
   uint64_t last = ~0ull;
   for (int i = 0; i < a.k; ++i) {
-    best = 0;
-    auto look = [&](float x, int id) {
-      const uint64_t k = top_key(x, id);
-      if (k < last && k > best) best = k;
-    };
-    for (v = tid; v < nv; v += THREADS) {
-      float x[N];
-      Row16<T>::open(Row16<T>::raw(z + (int64_t)v * N), x);
-#pragma unroll
-      for (int j = 0; j < N; ++j) look(x[j], v * N + j);
+    uint64_t top = 0;
+    for (int e = tid; e < a.V; e += THREADS) {
+      const uint64_t k = top_key(ld1<T>(z + e), e);
+      if (k < last && k > top) top = k;
     }
-    if (tail + tid < a.V) look(ld1<T>(z + tail + tid), tail + tid);
-    best = shfl_max64(best);
+    top = shfl_max64(top);
     __syncthreads();
-    if (lane == 0) wkey[wv] = best;
+    if (lane == 0) wkey[wv] = top;
     __syncthreads();
     last = wkey[0];
     for (int j = 1; j < W; ++j) last = wkey[j] > last ? wkey[j] : last;
@@ -292,7 +357,7 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
 
 constexpr int kBwdThreads = 256, kBwdU = 4;
 
-// grid (chunks, rows): a workgroup writes kBwdThreads * kBwdU 16-byte pieces of one row's gradient
+// A workgroup writes kBwdThreads * kBwdU 16-byte pieces of one row's gradient.
 template <typename T>
 __global__ __launch_bounds__(kBwdThreads) void token_lp_bwd_k(const LpArgs a, const float* __restrict__ dlogp,
                                                               const float* __restrict__ dent, T* __restrict__ dz,
@@ -331,7 +396,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_lp_bwd_k(const LpArgs a, co
     return;
   }
   const T* z = row_ptr<T>(a, row);
-  u32x4a r[kBwdU];
+  u32x4 r[kBwdU];
 #pragma unroll
   for (int i = 0; i < kBwdU; ++i) {
     const int v = v0 + i * kBwdThreads;
@@ -373,7 +438,7 @@ hipError_t token_logprobs_fwd(int dtype, const void* z, int64_t s0, int64_t s1, 
                               const int64_t* target, int64_t ignore, float inv_t, float* logp, float* ent, float* stats,
                               int k, float* top_lp, int64_t* top_id, hipStream_t stream) {
   if (rows == 0) return hipSuccess;
-  if (V < 1 || inner < 1 || k < 0 || k > kTokenTopMax || k > V || rows >= kTokenRowsMax) return hipErrorInvalidValue;
+  if (V < 1 || inner < 1 || k < 0 || k > kTokenTopMax || k > V || rows >= kTokenRowsMax || (k > 0 && V > kTokenTopVocab)) return hipErrorInvalidValue;
   LpArgs a = lp_args(z, s0, s1, inner, V, target, ignore, inv_t);
   a.logp = logp;
   a.ent = ent;
@@ -381,16 +446,23 @@ hipError_t token_logprobs_fwd(int dtype, const void* z, int64_t s0, int64_t s1, 
   a.k = k;
   a.top_lp = top_lp;
   a.top_id = top_id;
+  // Few rows: 1024 threads, so that one CU has a row's loads in flight at once.  Many rows: 256, eight workgroups a CU.
   const bool wide = rows < 512 && V > 8192;
+#define HYP_LP(TH, U, TOP)                                                                                             \
+  do {                                                                                                                 \
+    const int its = V / (Row16<T>::N * TH * U) + 1;                                                                    \
+    hipLaunchKernelGGL((token_lp_fwd_k<T, TH, U, TOP>), dim3(rows), dim3(TH), TOP ? its * TH * sizeof(float) : 0, stream, a); \
+  } while (0)
   HYP_DISPATCH_FLOAT(dtype, T, {
     if (k > 0) {
-      if (wide) hipLaunchKernelGGL((token_lp_fwd_k<T, 1024, true>), dim3(rows), dim3(1024), 0, stream, a);
-      else hipLaunchKernelGGL((token_lp_fwd_k<T, 256, true>), dim3(rows), dim3(256), 0, stream, a);
+      if (wide) HYP_LP(1024, 8, true);
+      else HYP_LP(256, (sizeof(T) == 4 ? 8 : 4), true);
     } else {
-      if (wide) hipLaunchKernelGGL((token_lp_fwd_k<T, 1024, false>), dim3(rows), dim3(1024), 0, stream, a);
-      else hipLaunchKernelGGL((token_lp_fwd_k<T, 256, false>), dim3(rows), dim3(256), 0, stream, a);
+      if (wide) HYP_LP(1024, 4, false);
+      else HYP_LP(256, 4, false);
     }
   });
+#undef HYP_LP
   return hipGetLastError();
 }
 

@@ -190,11 +190,12 @@ class _InferCtx:
         pass
 
 
-def apply_fn(fn, *args):
-    """``fn.apply(*args)``, or — with grad mode off (eval / inference) — ``fn.forward`` on a stand-in
+def apply_fn(fn, *args, needs_grad: bool = True):
+    """``fn.apply(*args)``, or — with grad mode off (eval / inference) or where the caller knows that no
+    argument needs a gradient (``needs_grad=False``) — ``fn.forward`` on a stand-in
     ctx: the same kernels without the autograd-node bookkeeping, which costs ~10 us of host time per
     op and made the launch-bound fused inference of LM-768 slower than torch eager."""
-    if torch.is_grad_enabled():
+    if needs_grad and torch.is_grad_enabled():
         return fn.apply(*args)
     return fn.forward(_InferCtx(), *args)
 

@@ -185,7 +185,8 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Tensor, bias: Optional[torch.Tens
         raise ValueError("mxfp4_linear: x, weight and bias must be on one device")
     if bias is not None and (bias.shape != (weight.shape[0],) or not bias.is_floating_point()):
         raise ValueError(f"mxfp4_linear: bias must be a floating [{weight.shape[0]}], got {tuple(bias.shape)} {bias.dtype}")
-    return _native.apply_fn(_MXLinearFn, x, bias, weight)
+    needs_grad = x.requires_grad or (bias is not None and bias.requires_grad)
+    return _native.apply_fn(_MXLinearFn, x, bias, weight, needs_grad=needs_grad)
 
 
 class MXFP4Linear(nn.Module):

@@ -26,6 +26,7 @@ from torch.autograd.function import once_differentiable
 from . import _native
 
 TOP_MAX = 32  # hyp::kTokenTopMax
+TOP_VOCAB = 1 << 18  # hyp::kTokenTopVocab
 
 
 class TokenLogprobs(NamedTuple):
@@ -86,8 +87,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
         else:
             rows = logits.reshape(-1, logits.shape[-1])
             lp, h, stats, tl, ti = _reference_fwd(rows, target.reshape(-1), k, ignore_index, inv_t)
-        lead = logits.shape[:-1]
-        lp, h, tl, ti = lp.view(lead), h.view(lead), tl.view(*lead, k), ti.view(*lead, k)
+            lead = logits.shape[:-1]
+            lp, h, tl, ti = lp.view(lead), h.view(lead), tl.view(*lead, k), ti.view(*lead, k)
         ctx.save_for_backward(logits, target, stats)
         ctx.cfg = (ignore_index, inv_t, native)
         ctx.mark_non_differentiable(tl, ti)
@@ -115,8 +116,8 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, i
                    temperature: float = 1.0) -> TokenLogprobs:
     """Scores ``target`` [...] under ``logits`` [..., V] (bf16, fp16 or fp32).
 
-    ``logprobs`` and ``entropy`` are differentiable in the logits (once); the ``top_k`` (at most 32)
-    alternatives are not.  Logits whose rows have unit stride are read where they are, whatever the
+    ``logprobs`` and ``entropy`` are differentiable in the logits (once); the ``top_k`` (at most 32, of at
+    most 2^18 tokens) alternatives are not.  Logits whose rows have unit stride are read where they are, whatever the
     strides of their (at most two) leading dimensions: ``logits[:, :-1]`` is not copied."""
     if logits.dtype not in _native.DTYPE_CODE:
         raise TypeError(f"token_logprobs: logits must be fp32, bf16 or fp16, got {logits.dtype}")
@@ -131,6 +132,8 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, i
     V = logits.shape[-1]
     if not 0 <= top_k <= min(TOP_MAX, V):
         raise ValueError(f"token_logprobs: top_k must be in [0, {min(TOP_MAX, V)}], got {top_k}")
+    if top_k and V > TOP_VOCAB:
+        raise ValueError(f"token_logprobs: alternatives are for at most {TOP_VOCAB} tokens, got {V}")
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"token_logprobs: temperature must be in [1e-6, 1e6], got {temperature}")
     if logits.dim() > 3 or (logits.stride(-1) != 1 and V > 1):
@@ -138,6 +141,6 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, i
         if logits.dim() > 3:
             out = token_logprobs(logits.view(-1, V), target.reshape(-1), top_k, ignore_index, temperature)
             return TokenLogprobs(*(None if t is None else t.view(*target.shape, *t.shape[1:]) for t in out))
-    lp, h, tl, ti = _native.apply_fn(_TokenLogprobsFn, logits, target.long().contiguous(), int(top_k), int(ignore_index),
-                                     1.0 / float(temperature))
+    args = (logits, target.long().contiguous(), int(top_k), int(ignore_index), 1.0 / float(temperature))
+    lp, h, tl, ti = _native.apply_fn(_TokenLogprobsFn, *args, needs_grad=logits.requires_grad)
     return TokenLogprobs(lp, h, tl if top_k else None, ti if top_k else None)

@@ -77,12 +77,57 @@ def test_ties_go_to_the_lowest_id(R):
 
 
 def test_more_candidates_than_fit():
-    # the first thread of every wave holds all of the row's largest logits: the bound passes thousands
+    # most threads' largest logit is small and a few hold thousands of large ones: the bound passes them all
     V = 130000
-    z = torch.zeros(1, V)
-    v = torch.arange(V) // 4
-    z[0] = torch.where(v % 64 < 2, torch.arange(V) % 997 * 1e-3 + 1, -torch.arange(V) * 1e-6)
+    z = -torch.arange(V)[None] * 1e-6
+    lot = torch.arange(V) // 8 % 1024 % 64 < 2
+    z[0, lot] = 1 + torch.arange(V)[lot] % 997 * 1e-3
     compare(z.to(DEV), torch.tensor([5]), torch.ones(1), torch.ones(1), 32)
+
+
+@pytest.mark.parametrize("value", [-math.inf, -1e9, 0.0])
+@pytest.mark.parametrize("R", [2, 515])
+def test_few_tokens_above_a_mask(R, value):
+    # fewer tokens above the mask's value than alternatives, in one place, at both ends, and with a lower one
+    V = 40000
+    z = torch.full((R, V), value)
+    z[0, 20000:20004] = torch.tensor([1.0, 3.0, 2.0, 3.0])
+    z[1, [0, 7, V - 1]] = torch.tensor([5.0, 4.0, 6.0])
+    if value != -math.inf:
+        z[1, 3] = -math.inf
+    t = torch.full((R,), 20001)
+    t[1] = V - 1
+    compare(z.to(DEV), t, torch.ones(R), torch.ones(R), 20)
+
+
+def test_ties_with_the_bound_far_behind():
+    # logits equal to the bound that the first ids do not hold
+    V = 60000
+    z = torch.full((1, V), -1.0)
+    z[0, 30000:] = 2.0
+    z[0, 59999] = 3.0
+    compare(z.to(DEV), torch.tensor([1]), torch.ones(1), torch.ones(1), 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_largest_vocabulary_with_alternatives(dtype):
+    z, t, a, b = rows(2, 1 << 18, dtype, 3)
+    compare(z.to(DEV), t, a, b, 32)
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(1, (1 << 18) + 1, device=DEV), torch.zeros(1, dtype=torch.long, device=DEV), top_k=1)
+
+
+@pytest.mark.parametrize("offset", range(8))
+def test_every_alignment(offset):
+    z, t, a, b = rows(1, 300 + offset, torch.bfloat16, offset)
+    buf = torch.empty(400, dtype=torch.bfloat16, device=DEV)
+    view = buf[offset:offset + 300 + offset].view(1, -1)
+    view.copy_(z)
+    compare(view, t, a, b, 7, ref=z)
+    zs, ts, a, b = rows(1, 3, torch.bfloat16, offset)
+    view = buf[offset:offset + 3].view(1, -1)
+    view.copy_(zs)
+    compare(view, ts, a, b, 3, ref=zs)
 
 
 def test_strided_views_are_read_in_place():
