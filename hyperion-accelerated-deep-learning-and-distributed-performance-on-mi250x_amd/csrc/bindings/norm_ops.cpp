@@ -197,6 +197,71 @@ void adam8_mt(const at::Tensor& ptrs, const at::Tensor& sizes, const at::Tensor&
                                         ptr_or_null<float>(found_inf), cur_stream(), zero_grad ? 1 : 0));
 }
 
+// What an optimizer step's launch tables depend on, as bytes: for every parameter of the groups its identity,
+// address, size and strides and (grads) those of the gradient that the step takes (main_grad, else grad); for every entry
+// of the state dict the parameter's identity and the addresses and sizes of the tensors under `keys`.  Two equal values
+// mean that the tables still fit (one pass in C++ instead of several over the tensors in Python).
+pybind11::bytes optim_fingerprint(const pybind11::list& groups, const pybind11::dict& state, const pybind11::tuple& keys,
+                                  bool grads) {
+  static PyObject* const kMain = PyUnicode_InternFromString("main_grad");
+  static PyObject* const kDict = PyUnicode_InternFromString("__dict__");
+  static PyObject* const kParams = PyUnicode_InternFromString("params");
+  std::vector<int64_t> v;
+  auto tensor = [&](PyObject* o) {
+    if (o == nullptr || !THPVariable_Check(o)) {
+      v.push_back(0);
+      v.push_back(-1);
+      return;
+    }
+    const at::Tensor& t = THPVariable_Unpack(o);
+    v.push_back((int64_t)t.const_data_ptr());
+    v.push_back(t.numel());
+  };
+  auto layout = [&](const at::Tensor& t) {
+    v.push_back((int64_t)t.const_data_ptr());
+    v.push_back((int64_t)t.scalar_type() | ((int64_t)t.dim() << 8));
+    for (int64_t n : t.sizes()) v.push_back(n);
+    for (int64_t n : t.strides()) v.push_back(n);
+  };
+  for (const auto& g : groups) {
+    PyObject* params = PyDict_GetItem(g.ptr(), kParams);
+    TORCH_CHECK(params != nullptr && PyList_Check(params), "optim_fingerprint: param groups with a list of params");
+    const Py_ssize_t n = PyList_GET_SIZE(params);
+    v.push_back(-1 - n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* p = PyList_GET_ITEM(params, i);
+      TORCH_CHECK(THPVariable_Check(p), "optim_fingerprint: params must be tensors");
+      const at::Tensor& t = THPVariable_Unpack(p);
+      v.push_back((int64_t)p);
+      layout(t);
+      if (!grads) continue;
+      PyObject* main = nullptr;
+      if (PyObject* d = PyObject_GetAttr(p, kDict)) {
+        main = PyDict_Check(d) ? PyDict_GetItem(d, kMain) : nullptr;
+        Py_DECREF(d);  // the parameter keeps it
+      } else {
+        PyErr_Clear();
+      }
+      if (main != nullptr && main != Py_None && THPVariable_Check(main)) {
+        v.push_back(1);
+        layout(THPVariable_Unpack(main));
+      } else if (t.grad().defined()) {
+        v.push_back(2);
+        layout(t.grad());
+      } else {
+        v.push_back(0);
+      }
+    }
+  }
+  Py_ssize_t pos = 0;
+  PyObject *p = nullptr, *st = nullptr;
+  while (PyDict_Next(state.ptr(), &pos, &p, &st)) {
+    v.push_back((int64_t)p);
+    for (const auto& k : keys) tensor(PyDict_Check(st) ? PyDict_GetItem(st, k.ptr()) : nullptr);
+  }
+  return pybind11::bytes(reinterpret_cast<const char*>(v.data()), v.size() * sizeof(int64_t));
+}
+
 // the moments of a table [m codes, v codes, m scales, v scales][T] as two dense fp32 vectors of `total` elements
 std::vector<at::Tensor> adam8_values(const at::Tensor& ptrs, const at::Tensor& sizes, const at::Tensor& blocks,
                                      const at::Tensor& offs, int64_t T, int64_t chunk, int64_t total) {
@@ -273,6 +338,8 @@ void register_norm_ops(pybind11::module& m) {
   m.def("bn_bwd_dx", &bn_bwd_dx, "BN backward dx pass from a pre-masked dz and its complete sums");
   m.def("adam_mt", &adam_mt, "multi-tensor fused Adam/AdamW");
   m.def("adam8_mt", &adam8_mt, "multi-tensor fused Adam/AdamW with 8-bit moments");
+  m.def("optim_fingerprint", &optim_fingerprint, "what an optimizer step's launch tables depend on, as bytes",
+        pybind11::arg("groups"), pybind11::arg("state"), pybind11::arg("keys"), pybind11::arg("grads"));
   m.def("adam8_values", &adam8_values, "8-bit moments of a table as dense fp32 vectors");
   m.def("adam_set_streaming", [](int64_t on) { hyp::adam_set_streaming((int)on); },
         "A/B: non-temporal loads / stores of the fp32 optimizer state in adam_mt");

@@ -140,10 +140,15 @@ class TableCache:
             else:
                 t = MultiTensorTable(groups)  # raises under capture (no allocation in the graph pool)
             self._tables[role] = t
-        if capturing and not getattr(t, "pinned", False):
+        if capturing:
+            self.pin(role, t)
+        return t
+
+    def pin(self, role: str, t: MultiTensorTable) -> None:
+        """Keeps ``t`` as it is from now on: a capture uses it."""
+        if not getattr(t, "pinned", False):
             t.pinned = True
             self._pinned.setdefault(role, []).append(t)
-        return t
 
     def pinned(self) -> List[MultiTensorTable]:
         return [t for ts in self._pinned.values() for t in ts]

@@ -128,3 +128,66 @@ def test_other_stream_and_graph_replays():
 
 def test_many_small_tensors_in_one_launch():
     run_against_oracle([(17, i % 9 + 1) for i in range(120)], torch.bfloat16, DEV, steps=2)
+
+
+def test_tables_follow_what_changes_between_steps():
+    """Steps replay the last one's tables where nothing changed: new gradients, frozen and thawed parameters, replaced
+    state, a loaded checkpoint, main_grad and new hyperparameters are all noticed."""
+    torch.manual_seed(3)
+    ws = [torch.randn(400, device=DEV), torch.randn(31, 9, device=DEV)]
+    native = [torch.nn.Parameter(w.clone()) for w in ws]
+    plain = [torch.nn.Parameter(w.cpu()) for w in ws]
+    a, b = FusedAdamW(native, lr=1e-2, state_bits=8), FusedAdamW(plain, lr=1e-2, state_bits=8)
+
+    def step(which=(0, 1), main=False, keep=False):
+        for i, (p, q) in enumerate(zip(native, plain)):
+            if i not in which:
+                p.grad = q.grad = None
+                continue
+            g = torch.randn(q.shape)
+            if main:
+                p.main_grad, q.main_grad = g.to(DEV), g.clone()
+            elif keep and p.grad is not None:
+                p.grad.copy_(g), q.grad.copy_(g)
+            else:
+                p.grad, q.grad = g.to(DEV), g.clone()
+        a.step(), b.step()
+        for p, q in zip(native, plain):
+            for k in ("exp_avg_q", "exp_avg_sq_q", "exp_avg_scale", "exp_avg_sq_scale"):
+                assert torch.equal(a.state[p][k].cpu(), b.state[q][k]) if a.state.get(p) else not b.state.get(q)
+            torch.testing.assert_close(p.detach().cpu(), q.detach(), rtol=1e-6, atol=1e-7)
+        assert all(torch.equal(x.cpu(), y) for x, y in zip(a.moment_vectors(), b.moment_vectors()))
+
+    step(which=(0,))
+    for _ in range(3):
+        step(keep=True)
+    held = [p.grad for p in native]
+    step()
+    step(which=(1,))
+    step(keep=True)
+    for o, ps in ((a, native), (b, plain)):
+        o.state[ps[0]]["exp_avg_q"] = torch.full_like(o.state[ps[0]]["exp_avg_q"], 5)
+        o.param_groups[0]["lr"] = 3e-2
+        o.param_groups[0]["weight_decay"] = 0.2
+    step(keep=True)
+    sa, sb = a.state_dict(), b.state_dict()
+    step(keep=True)
+    a.load_state_dict(sa), b.load_state_dict(sb)
+    step(keep=True)
+    step(main=True)
+    step(main=True)
+    for p, q in zip(native, plain):
+        del p.main_grad, q.main_grad
+    step(keep=True)
+    assert held
+
+
+def test_steps_without_changes_do_not_walk_the_tensors(monkeypatch):
+    ps = [torch.nn.Parameter(torch.randn(64, device=DEV)) for _ in range(4)]
+    for p in ps:
+        p.grad = torch.randn_like(p)
+    opt = FusedAdamW(ps, state_bits=8)
+    opt.step(), opt.moment_vectors()
+    monkeypatch.setattr(opt, "_step8", None)
+    monkeypatch.setattr(opt._tables, "get", None)
+    opt.step(), opt.moment_vectors()
