@@ -38,6 +38,14 @@ struct Adam8Args {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
+// a tensor's address out of a table: global memory (the compiler would have to use flat accesses, which also
+// occupy the LDS counter)
+template <typename T>
+__device__ __forceinline__ T* table_ptr(int64_t a) {
+  typedef __attribute__((address_space(1))) T G;
+  return (T*)reinterpret_cast<G*>(a);
+}
+
 template <typename T>
 __device__ __forceinline__ void load_lane(const T* p, int left, float (&v)[8]) {
   if (left >= 8) {
@@ -106,18 +114,18 @@ __global__ __launch_bounds__(kThreads) void adam8_mt_k(const int64_t* __restrict
   const int t = blocks[2 * blockIdx.x], ck = blocks[2 * blockIdx.x + 1];
   const int64_t n = sizes[t];
   const int64_t start = (int64_t)ck * chunk, end = min(n, start + chunk);
-  G* g = reinterpret_cast<G*>(ptrs[T + t]);
+  G* g = table_ptr<G>(ptrs[T + t]);
   if (found_inf != nullptr && *found_inf != 0.f) {  // an overflowed step is skipped
     if (a.zero_grad)
       for (int64_t i = start + threadIdx.x; i < end; i += kThreads) st1<G>(g + i, 0.f);
     return;
   }
-  PL* pl = reinterpret_cast<PL*>(ptrs[t]);
-  float* p = reinterpret_cast<float*>(MASTER ? ptrs[6 * T + t] : ptrs[t]);
-  uint8_t* mq = reinterpret_cast<uint8_t*>(ptrs[2 * T + t]);
-  uint8_t* vq = reinterpret_cast<uint8_t*>(ptrs[3 * T + t]);
-  float* ms = reinterpret_cast<float*>(ptrs[4 * T + t]);
-  float* vs = reinterpret_cast<float*>(ptrs[5 * T + t]);
+  PL* pl = table_ptr<PL>(ptrs[t]);
+  float* p = table_ptr<float>(MASTER ? ptrs[6 * T + t] : ptrs[t]);
+  uint8_t* mq = table_ptr<uint8_t>(ptrs[2 * T + t]);
+  uint8_t* vq = table_ptr<uint8_t>(ptrs[3 * T + t]);
+  float* ms = table_ptr<float>(ptrs[4 * T + t]);
+  float* vs = table_ptr<float>(ptrs[5 * T + t]);
   const float step = *step_t;
   const float lr = lr_t ? *lr_t : a.lr, gs = inv_scale ? *inv_scale : 1.f;
   const float lr1 = lr / -expm1f(step * a.ln_b1), rb2 = rsqrtf(-expm1f(step * a.ln_b2));
@@ -148,7 +156,7 @@ __global__ __launch_bounds__(kThreads) void adam8_mt_k(const int64_t* __restrict
       m_top = max(m_top, __float_as_uint(mf) & 0x7fffffffu);
       v_top = max(v_top, __float_as_uint(vf) & 0x7fffffffu);
       if (a.adamw) pv[i] = fmaf(-decay, pv[i], pv[i]);
-      pv[i] = fmaf(-lr1, mf / fmaf(__builtin_amdgcn_sqrtf(vf), rb2, a.eps), pv[i]);
+      pv[i] = fmaf(-lr1 * mf, __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(vf), rb2, a.eps)), pv[i]);
     }
     const float m_s = kept_scale(half_max(m_top)), v_s = kept_scale(half_max(v_top));
     const bool m_live = m_s > 0.f, v_live = v_s > 0.f;  // neither 0 nor NaN
@@ -157,22 +165,18 @@ __global__ __launch_bounds__(kThreads) void adam8_mt_k(const int64_t* __restrict
     uint32_t mo[2] = {0u, 0u}, vo[2] = {0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (m_live) {
-        const double x = fabs(md[i]);
-        const float k = fminf(floorf(__builtin_amdgcn_sqrtf((float)x * m_inv) * 127.f), 127.f);
-        const int q = (int)k + (x > m_unit * (double)(fmaf(k, k, k) + 0.25f));
-        mo[i >> 2] |= ((unsigned)(md[i] < 0.0 ? -q : q) & 255u) << (8 * (i & 3));
-      }
-      if (v_live) {
-        const double x = vd[i];
-        const float r = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)x * v_inv));
-        const float k = fminf(floorf(r * 255.f), 255.f), h = k + 0.5f;
-        const double h2 = (double)(h * h);
-        unsigned q = (unsigned)k + (x > v_unit * (h2 * h2));
-        if (q == 0u && x > 0.0) q = 1u;
-        vo[i >> 2] |= q << (8 * (i & 3));
-      }
+      const double x = fabs(md[i]), y = vd[i];
+      const float km = fminf(floorf(__builtin_amdgcn_sqrtf((float)x * m_inv) * 127.f), 127.f);
+      const int qm = (int)km + (x > m_unit * (double)(fmaf(km, km, km) + 0.25f));
+      mo[i >> 2] |= ((unsigned)(md[i] < 0.0 ? -qm : qm) & 255u) << (8 * (i & 3));
+      const float r = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y * v_inv));
+      const float kv = fminf(floorf(r * 255.f), 255.f), h = kv + 0.5f;
+      const double h2 = (double)(h * h);
+      const unsigned qv = (unsigned)kv + (y > v_unit * (h2 * h2));
+      vo[i >> 2] |= (qv == 0u && y > 0.0 ? 1u : qv) << (8 * (i & 3));
     }
+    if (!m_live) mo[0] = mo[1] = 0u;
+    if (!v_live) vo[0] = vo[1] = 0u;
     if (left > 0) {
       store_lane<float>(p + i0, left, pv);
       if (MASTER) store_lane<PL>(pl + i0, left, pv);
@@ -197,10 +201,10 @@ __global__ __launch_bounds__(kThreads) void adam8_values_k(const int64_t* __rest
   const int t = blocks[2 * blockIdx.x], ck = blocks[2 * blockIdx.x + 1];
   const int64_t n = sizes[t];
   const int64_t start = (int64_t)ck * chunk, end = min(n, start + chunk), at = offs[t];
-  const uint8_t* mq = reinterpret_cast<const uint8_t*>(ptrs[t]);
-  const uint8_t* vq = reinterpret_cast<const uint8_t*>(ptrs[T + t]);
-  const float* ms = reinterpret_cast<const float*>(ptrs[2 * T + t]);
-  const float* vs = reinterpret_cast<const float*>(ptrs[3 * T + t]);
+  const uint8_t* mq = table_ptr<const uint8_t>(ptrs[t]);
+  const uint8_t* vq = table_ptr<const uint8_t>(ptrs[T + t]);
+  const float* ms = table_ptr<const float>(ptrs[2 * T + t]);
+  const float* vs = table_ptr<const float>(ptrs[3 * T + t]);
   for (int64_t i0 = start + threadIdx.x * 4; i0 < end; i0 += kThreads * 4) {
     const int left = (int)min((int64_t)4, end - i0);
     uint32_t mw = 0, vw = 0;
