@@ -20,8 +20,7 @@
 //
 // A half wave holds one block, 8 elements a lane; the block's maxima meet over the 32 lanes by lane
 // exchanges in registers.  Per element: gradient 2 or 4 bytes, fp32 parameter 4 + 4 (+ 2 its bf16 / fp16
-// copy), codes 2 + 2, scales 16 / 256.  Measured (MI355X): 180M bf16 parameters with masters 590 us (4.9 TB/s, a
-// large copy's rate is 5.1), 16.8M in 256 tensors 59 us; about 80 VALU slots an element keep the lanes as busy as HBM.
+// copy), codes 2 + 2, scales 16 / 256.
 #include "hyp_common.h"
 #include "hyp_kernels.h"
 
@@ -64,27 +63,6 @@ __device__ __forceinline__ void store_lane(T* p, int left, const float (&v)[8]) 
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < left) st1<T>(p + i, v[i]);
-  }
-}
-// fp32 masters are read and written once a step and by nothing else: past the caches (180M parameters: 614 -> 590 us)
-__device__ __forceinline__ void load_master(const float* p, int left, float (&v)[8]) {
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  if (left < 8) return load_lane<float>(p, left, v);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const u32x4 r = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + h);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[4 * h + i] = __uint_as_float(r[i]);
-  }
-}
-__device__ __forceinline__ void store_master(float* p, int left, const float (&v)[8]) {
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  if (left < 8) return store_lane<float>(p, left, v);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const u32x4 r = {__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]),
-                     __float_as_uint(v[4 * h + 3])};
-    __builtin_nontemporal_store(r, reinterpret_cast<u32x4*>(p) + h);
   }
 }
 __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int left) {
@@ -159,8 +137,7 @@ __global__ __launch_bounds__(kThreads) void adam8_mt_k(const int64_t* __restrict
     const int left = (int)min((int64_t)8, end - i0);  // <= 0 behind the end
     float pv[8], gv[8];
     uint2 mw = make_uint2(0u, 0u), vw = make_uint2(0u, 0u);
-    if (MASTER) load_master(p + i0, left, pv);
-    else load_lane<float>(p + i0, left, pv);
+    load_lane<float>(p + i0, left, pv);
     load_lane<G>(g + i0, left, gv);
     mw = load_codes(mq + i0, left);
     vw = load_codes(vq + i0, left);
@@ -201,12 +178,8 @@ __global__ __launch_bounds__(kThreads) void adam8_mt_k(const int64_t* __restrict
     if (!m_live) mo[0] = mo[1] = 0u;
     if (!v_live) vo[0] = vo[1] = 0u;
     if (left > 0) {
-      if (MASTER) {
-        store_master(p + i0, left, pv);
-        store_lane<PL>(pl + i0, left, pv);
-      } else {
-        store_lane<float>(p + i0, left, pv);
-      }
+      store_lane<float>(p + i0, left, pv);
+      if (MASTER) store_lane<PL>(pl + i0, left, pv);
       if (a.zero_grad) {
         const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         store_lane<G>(g + i0, left, zero);
