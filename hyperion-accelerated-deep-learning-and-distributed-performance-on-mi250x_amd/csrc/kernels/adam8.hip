@@ -20,7 +20,9 @@
 //
 // A half wave holds one block, 8 elements a lane; the block's maxima meet over the 32 lanes by lane
 // exchanges in registers.  Per element: gradient 2 or 4 bytes, fp32 parameter 4 + 4 (+ 2 its bf16 / fp16
-// copy), codes 2 + 2, scales 16 / 256.
+// copy), codes 2 + 2, scales 16 / 256.  Measured (MI355X): 180M bf16 parameters with masters 614 us (4.7 TB/s; a large copy
+// reaches 5.1), 16.8M in 256 tensors 58 us, 6.8M fp32 in 52 tensors 28 us.  About 80 VALU slots an element keep the
+// lanes nearly as busy as HBM; accesses of the masters past the caches gained 2% of the first, lost 7% of the second.
 #include "hyp_common.h"
 #include "hyp_kernels.h"
 
