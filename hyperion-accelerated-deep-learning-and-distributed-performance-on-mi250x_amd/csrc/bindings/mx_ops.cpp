@@ -114,6 +114,10 @@ void check_rows(const at::Tensor& x, const at::Tensor& codes, int64_t n, const c
               who, ": x [M, ", n, "] with unit column stride on the weight's device, all sizes in [1, 2^24)");
 }
 
+bool lds_ok(const at::Tensor& scales) {
+  return scales.size(1) % 4 == 0 && reinterpret_cast<uintptr_t>(scales.data_ptr()) % 4 == 0;
+}
+
 at::Tensor decoded(const at::Tensor& codes, const at::Tensor& scales) {
   return mx_dequantize(codes, scales, scales.size(1) * 32, at::kBFloat16);
 }
@@ -130,7 +134,7 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& codes, const at::Ten
   const at::Tensor xp = pieces(x, 32 * nb);
   const auto dt = P == 1 ? at::kBFloat16 : at::kFloat;
   int mt, nt;
-  hyp::mx_nt_plan((int)(P * M), (int)N, (int)nb, &mt, &nt);
+  hyp::mx_nt_plan((int)(P * M), (int)N, (int)nb, lds_ok(scales), &mt, &nt);
   if (tile >= 0) mt = (int)tile / 16, nt = (int)tile % 16;
   at::Tensor y;
   if (mt > 0) {
@@ -154,11 +158,12 @@ at::Tensor mx_linear_dgrad(const at::Tensor& dy, const at::Tensor& codes, const 
   TORCH_CHECK(K >= 1 && K < (1 << 24), "mx_linear_dgrad: K in [1, 2^24)");
   const at::DeviceGuard guard(dy.device());
   const int64_t M = dy.size(0), N = codes.size(0), nb = scales.size(1), P = pieces_of(dy.scalar_type());
-  const at::Tensor dp = pieces(dy, (N + 7) / 8 * 8);
   const auto dt = P == 1 ? at::kBFloat16 : at::kFloat;
   int mt;
-  hyp::mx_nn_plan((int)(P * M), (int)N, (int)nb, &mt);
+  hyp::mx_nn_plan((int)(P * M), (int)N, (int)nb, lds_ok(scales), &mt);
   if (tile >= 0) mt = (int)tile;
+  const int64_t unit = mt > hyp::kMxLds ? 128 : 8;  // the product through LDS takes whole groups of the reduction
+  const at::Tensor dp = pieces(dy, (N + unit - 1) / unit * unit);
   at::Tensor dx;
   if (mt > 0) {
     dx = at::empty({P * M, K}, dp.options().dtype(dt));

@@ -168,18 +168,19 @@ hipError_t mx_pieces(int dtype, const void* x, int64_t ld, int64_t rows, int col
 hipError_t mx_join(int dtype, const float* part, int pieces, int64_t rows, int cols, int64_t pitch, const float* bias,
                    void* y, hipStream_t stream);
 // y [M, N] (bf16 / fp32) = x [M, 32 nb] (bf16) times the transpose of the 4-bit weight [N, 32 nb] (+ bias), in tiles
-// of 16 mt x 16 nt, mt x nt one of 1x1 1x2 2x2 2x4 4x4
+// of 16 mt x 16 nt: 1x1 or 2x4, or through LDS (mt + kMxLds; nb % 4 == 0 and 4-byte aligned scales) 1x1 1x2 1x4 2x2 2x4
+constexpr int kMxLds = 8;
 hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
                  int out_dtype, void* y, hipStream_t stream, int mt, int nt);
-// the tile of mx_nt / mx_nn for a product, 0 where decoding the weight and the tiled GEMM are faster; the tiled GEMM's
-// (tile, splits) for it
-void mx_nt_plan(int M, int N, int nb, int* mt, int* nt);
-void mx_nn_plan(int M, int N, int nb, int* mt);
-void mx_gemm_plan(int M, int N, int K, int* tile, int* splits);
-// y [M, cols] (bf16 / fp32) = x [M, N] (bf16; rows of stride ld % 8 == 0, zeros from N to the next multiple of 8) times
-// the 4-bit weight [N, 32 nb], in tiles of 16 mt x 128, mt 1 or 2
+// y [M, cols] (bf16 / fp32) = x [M, N] (bf16; rows of stride ld, zeros from N to it) times the 4-bit weight [N, 32 nb], in
+// tiles of 16 mt x 128: mt 1 (ld % 8 == 0), or through LDS (mt + kMxLds; also ld % 128 == 0) 1 or 2
 hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, int cols,
                  int out_dtype, void* y, hipStream_t stream, int mt);
+// the tile of mx_nt / mx_nn for a product, 0 where decoding the weight and the tiled GEMM are faster (lds: the weight
+// allows the products through LDS); the tiled GEMM's (tile, splits) for it and their time in us
+void mx_nt_plan(int M, int N, int nb, bool lds, int* mt, int* nt);
+void mx_nn_plan(int M, int N, int nb, bool lds, int* mt);
+double mx_gemm_plan(int M, int N, int K, int* tile, int* splits);
 }  // namespace hyp
 
 namespace hyp {

@@ -9,6 +9,9 @@
 //
 // gfx950 converts both ways with the scale applied (v_cvt_scalef32_pk_*): two elements an
 // instruction, rounding and saturating as above, exact for all 256 scale bytes (0 and 255 among them).
+#include <algorithm>
+#include <cmath>
+
 #include "hyp_common.h"
 #include "hyp_kernels.h"
 #include "mfma_lds.h"
@@ -21,6 +24,7 @@ using mfl::u16x8;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -169,8 +173,7 @@ __global__ __launch_bounds__(kQThreads) void mx_join_k(const float* __restrict__
 // l & 15) without LDS or barriers in their loops: the waves of a workgroup share one output tile and
 // split its reduction into contiguous ranges, so that thin products still fill the chip, every wave
 // streams its own operands from L2, and one launch does it.  The partial tiles meet in LDS in wave order
-// (the result does not depend on timing).  Workgroups of one weight tile and different rows are 8 ids
-// apart, on one XCD: the weight comes from HBM once.
+// (the result does not depend on timing).
 constexpr int kMxWaves = 8;
 
 struct MxArgs {
@@ -182,20 +185,23 @@ struct MxArgs {
   int M, N, nb;  // weight [N, 32 nb]
   int cols;      // NN: columns of y (K of the weight)
   int64_t ld;    // NN: row stride of x
+  int group;     // row blocks of a group (mx_tile)
 };
 
-// workgroup -> (row block, weight tile)
-__device__ __forceinline__ void mx_tile(int rows, int tiles, int* mb, int* tile) {
-  const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
-  *mb = i % rows;
-  *tile = (i / rows) * 8 + xcd;
+// workgroup -> (row block, weight tile): every XCD takes a contiguous piece of the order row group, weight tile, row
+// block of the group.  A group's activations (at most 2 MB) and the piece's weight tiles stay in the XCD's L2.
+__device__ __forceinline__ void mx_tile(const MxArgs& a, int rows, int tiles, int* mb, int* tile) {
+  const int id = mfl::xcd_remap(blockIdx.x, gridDim.x);
+  const int group = id / (a.group * tiles), r = id - group * a.group * tiles;
+  const int size = min(a.group, rows - group * a.group);
+  *tile = r / size;
+  *mb = group * a.group + r % size;
 }
 
 // Lanes 16 g + l hold words w[0..3] of block g of row l; afterwards word j is word g of block j (a 4 x 4
 // transposition over the lane groups): reduction elements 8 g .. 8 g + 7 of block j, as the matrix
 // instruction wants them, so that the activations are read in rows of 64 bytes.
 __device__ __forceinline__ void mx_group_transpose(u32x4& w) {
-  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
   const u32x2 a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
   const u32x2 b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
   const u32x2 c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
@@ -234,9 +240,8 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_nt_k(const MxArgs a) {
   extern __shared__ float part[];  // [waves][MT][NT][256]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
   int mb, tile;
-  mx_tile((a.M + 16 * MT - 1) / (16 * MT), (a.N + 16 * NT - 1) / (16 * NT), &mb, &tile);
+  mx_tile(a, (a.M + 16 * MT - 1) / (16 * MT), (a.N + 16 * NT - 1) / (16 * NT), &mb, &tile);
   const int n0 = tile * 16 * NT, m0 = mb * 16 * MT;
-  if (n0 >= a.N) return;  // the last ids of a tile count that is no multiple of 8
   const int64_t K = (int64_t)a.nb * kMxBlock;
   const int groups = (a.nb + 3) >> 2;
   const int kb = (int)((int64_t)wave * groups / kMxWaves), ke = (int)((int64_t)(wave + 1) * groups / kMxWaves);
@@ -317,18 +322,183 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_nt_k(const MxArgs a) {
   }
 }
 
-// y [M, cols] = x W, x [M, N]: the reduction runs over the weight's rows.  A workgroup owns 16 MT rows and 128
+// ---- the same product through LDS --------------------------------------------------------------------------
+// Lanes 16 apart hold one row's neighbours in a fragment, so a fragment loaded from memory asks for 64 single 16-byte
+// pieces (64 clocks a KiB of a CU's 16).  Where rows are whole groups of four blocks, each wave therefore moves its
+// own operands with LDS-DMA, 256 contiguous bytes of an activation row and 64 of a weight row at a time, into a ring
+// of its own (no barrier in the loop), and reads the fragments from there.  Lane group g takes block g of the group:
+// one scale a lane and no exchange; the activation's fragment of step q is chunk 4 g + q of its row.
+// Images: activations [16 MT rows][16 chunks], chunk c of row r at slot c ^ h(r), h = the low four bits of r with
+// their halves swapped; weight [16 NT rows][4 chunks], chunk c of row r at c ^ f(r >> 2 & 3), f = 0 2 3 1; scales
+// [64 rows] of 4 bytes.  Both make every group of lanes that LDS serves at once touch 64 different banks.
+constexpr int kLdsWaves = 4;
+
+template <int N>
+__device__ __forceinline__ void mx_wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+
+__device__ __forceinline__ void lds_dma16(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+__device__ __forceinline__ void lds_dma4(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
+}
+
+// Fragment reads as asm, each block with its own wait (the compiler would wait for the whole ring before an LDS read).
+// four chunks of one 16-row image; the image begins OFF bytes behind the lane addresses
+template <int OFF>
+__device__ __forceinline__ void mx_read_x1(const unsigned (&ad)[4], u32x4 (&x)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %4 offset:%8\n\tds_read_b128 %1, %5 offset:%8\n\tds_read_b128 %2, %6 offset:%8\n\t"
+      "ds_read_b128 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+      : "v"(ad[0]), "v"(ad[1]), "v"(ad[2]), "v"(ad[3]), "i"(OFF)
+      : "memory");
+}
+__device__ __forceinline__ void mx_read_x2(const unsigned (&ad)[4], u32x4 (&x)[2][4]) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+      "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %10 offset:4096\n\t"
+      "ds_read_b128 %7, %11 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3]), "=&v"(x[1][0]), "=&v"(x[1][1]),
+        "=&v"(x[1][2]), "=&v"(x[1][3])
+      : "v"(ad[0]), "v"(ad[1]), "v"(ad[2]), "v"(ad[3])
+      : "memory");
+}
+__device__ __forceinline__ void mx_read_w(unsigned wa, unsigned sa, u32x4 (&w)[1], unsigned (&s)[1]) {
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b32 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(w[0]), "=&v"(s[0])
+               : "v"(wa), "v"(sa)
+               : "memory");
+}
+__device__ __forceinline__ void mx_read_w(unsigned wa, unsigned sa, u32x4 (&w)[2], unsigned (&s)[2]) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b32 %2, %5\n\tds_read_b32 %3, %5 offset:64\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(s[0]), "=&v"(s[1])
+      : "v"(wa), "v"(sa)
+      : "memory");
+}
+__device__ __forceinline__ void mx_read_w(unsigned wa, unsigned sa, u32x4 (&w)[4], unsigned (&s)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b128 %2, %8 offset:2048\n\t"
+      "ds_read_b128 %3, %8 offset:3072\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:64\n\t"
+      "ds_read_b32 %6, %9 offset:128\n\tds_read_b32 %7, %9 offset:192\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+      : "v"(wa), "v"(sa)
+      : "memory");
+}
+
+template <int MT, int NT>
+constexpr int mx_nt_lds_bytes(int stages) {
+  return kLdsWaves * stages * (MT * 4096 + NT * 1024 + 256);
+}
+
+template <int MT, int NT, int S, typename O>
+__global__ __launch_bounds__(kLdsWaves * 64) void mx_nt_lds_k(const MxArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int kX = MT * 4096, kW = NT * 1024, kStage = kX + kW + 256;
+  constexpr int L = MT * 4 + NT + 1;  // DMA instructions of a stage
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+  int mb, tile;
+  mx_tile(a, (a.M + 16 * MT - 1) / (16 * MT), (a.N + 16 * NT - 1) / (16 * NT), &mb, &tile);
+  const int n0 = tile * 16 * NT, m0 = mb * 16 * MT;
+  const int64_t K = (int64_t)a.nb * kMxBlock;
+  const int groups = a.nb >> 2;
+  const int kb = (int)((int64_t)wave * groups / kLdsWaves), n = (int)((int64_t)(wave + 1) * groups / kLdsWaves) - kb;
+  uint8_t* ring = lds + wave * (S * kStage);
+  // rows behind the ends read the last row: their outputs are not stored
+  const uint8_t* xs[MT * 4];
+  const uint8_t* ws[NT];
+#pragma unroll
+  for (int i = 0; i < MT * 4; ++i) {
+    const int r = 4 * i + (lane >> 4), m = min(m0 + r, a.M - 1);
+    const int h = ((r & 3) << 2) | ((r >> 2) & 3);
+    xs[i] = reinterpret_cast<const uint8_t*>(a.x + m * K) + kb * 256 + ((l15 ^ h) << 4);
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int r = lane >> 2, nn = min(n0 + 16 * j + r, a.N - 1);
+    ws[j] = a.codes + ((int64_t)nn * a.nb + kb * 4 + ((lane & 3) ^ ((0x78 >> (2 * (r >> 2))) & 3))) * 16;
+  }
+  const uint8_t* ss = a.scales + (int64_t)min(n0 + min(lane, 16 * NT - 1), a.N - 1) * a.nb + kb * 4;
+  auto issue = [&](int t) {
+    uint8_t* st = ring + (t % S) * kStage;
+#pragma unroll
+    for (int i = 0; i < MT * 4; ++i) lds_dma16(xs[i] + t * 256, st + i * 1024);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) lds_dma16(ws[j] + t * 64, st + kX + j * 1024);
+    lds_dma4(ss + t * 4, st + kX + kW);
+  };
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int h = ((l15 & 3) << 2) | (l15 >> 2);
+  const unsigned base = mfl::lds_addr(ring);
+  for (int t = 0; t < S - 1 && t < n; ++t) issue(t);
+  for (int t = 0; t < n; ++t) {
+    if (t + S - 1 < n) issue(t + S - 1);
+    const int ahead = n - 1 - t;
+    if (ahead >= S - 1) mx_wait_vm<(S - 1) * L>();
+    else if (S > 2 && ahead == 1) mx_wait_vm<L>();
+    else mx_wait_vm<0>();
+    const unsigned sb = base + (t % S) * kStage;
+    unsigned xa[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) xa[q] = sb + l15 * 256 + (((4 * g + q) ^ h) << 4);
+    u32x4 w[NT], x[MT][4];
+    unsigned sc[NT];
+    mx_read_w(sb + kX + l15 * 64 + ((g ^ ((0x78 >> (2 * (l15 >> 2))) & 3)) << 4), sb + kX + kW + l15 * 4, w, sc);
+    if constexpr (MT == 2) mx_read_x2(xa, x);
+    else mx_read_x1<0>(xa, x[0]);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const float s = mx_scale((sc[j] >> (8 * g)) & 255u);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const u16x8 f = mx_fragment(w[j][q], s);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = mfl::mma16<bf16_t>(__builtin_bit_cast(u16x8, x[i][q]), f, acc[i][j]);
+      }
+    }
+  }
+  __syncthreads();  // the rings become the partial tiles
+  constexpr int kTile = MT * NT * 256;
+  float* part = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave * kTile + (16 * i + 4 * g + e) * (16 * NT) + 16 * j + l15] = acc[i][j][e];
+  __syncthreads();
+  O* y = static_cast<O*>(a.y);
+  for (int t = threadIdx.x; t < kTile; t += kLdsWaves * 64) {
+    const int m = m0 + t / (16 * NT), c = n0 + t % (16 * NT);
+    if (m >= a.M || c >= a.N) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kLdsWaves; ++w) sum += part[w * kTile + t];
+    if (a.bias) sum += a.bias[c];
+    st1<O>(y + (int64_t)m * a.N + c, sum);
+  }
+}
+
+// y [M, cols] = x W, x [M, N]: the reduction runs over the weight's rows.  A workgroup owns 16 rows and 128
 // columns, 32 weight rows a step: a lane loads 8 elements (4 bytes) of each of 8 weight rows, decodes them
 // under each row's own scale and transposes the 8 x 8 in registers (v_perm), which gives the fragments of
 // columns 8 (l & 15) + c, c = 0..7: no transposed copy of the weight, and 16 consecutive bytes of y a lane.
-template <int MT, typename O>
+template <typename O>
 __global__ __launch_bounds__(kMxWaves * 64) void mx_nn_k(const MxArgs a) {
-  extern __shared__ float part[];  // [waves][16 MT][128]
+  constexpr int MT = 1;
+  extern __shared__ float part[];  // [waves][16][128]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
   int mb, tile;
-  mx_tile((a.M + 16 * MT - 1) / (16 * MT), (a.cols + 127) / 128, &mb, &tile);
+  mx_tile(a, (a.M + 16 * MT - 1) / (16 * MT), (a.cols + 127) / 128, &mb, &tile);
   const int k0 = tile * 128, m0 = mb * 16 * MT;
-  if (k0 >= a.cols) return;
   const int steps = (a.N + 31) >> 5;
   const int sb = (int)((int64_t)wave * steps / kMxWaves), se = (int)((int64_t)(wave + 1) * steps / kMxWaves);
   const int blk = (k0 >> 5) + (l15 >> 2);
@@ -411,6 +581,184 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_nn_k(const MxArgs a) {
   }
 }
 
+// ---- the data gradient through LDS ------------------------------------------------------------------------
+// y [M, cols] = x W, x [M, ld] with zeros from N to ld, a multiple of 128: the reduction runs over the weight's rows, 128 a
+// stage.  A workgroup owns 16 MT rows and 128 columns; the waves split the reduction and each fills a ring of its own as
+// above.  A lane reads 8 elements (4 bytes) of each of 8 weight rows, decodes them under each row's own scale
+// and transposes the 8 x 8 in registers (v_perm), which gives the fragments of columns 8 (l & 15) + c, c = 0..7:
+// no transposed copy of the weight, and 32 consecutive bytes of the partial tile a lane.  The decoding, about
+// 80 instructions for 32 rows, is what bounds it up to 32 rows of x.
+// Images: activations as above with h(r) = r; weight rows 8 g + r of every 32 at place 4 r + g, 64 bytes each, so
+// that the four lane groups read 256 consecutive bytes; scales [128 rows] of 4 bytes.
+template <int S0>
+__device__ __forceinline__ void mx_read_nn(unsigned wa, unsigned sa, unsigned xa0, unsigned xa1, u32x2 (&w)[8], u32x4 (&s)[4],
+                                           u32x4 (&x)[1][2]) {
+  asm volatile(
+      "ds_read2st64_b32 %0, %14 offset0:%18 offset1:%19\n\t"
+      "ds_read2st64_b32 %1, %14 offset0:%20 offset1:%21\n\t"
+      "ds_read2st64_b32 %2, %14 offset0:%22 offset1:%23\n\t"
+      "ds_read2st64_b32 %3, %14 offset0:%24 offset1:%25\n\t"
+      "ds_read2st64_b32 %4, %14 offset0:%26 offset1:%27\n\t"
+      "ds_read2st64_b32 %5, %14 offset0:%28 offset1:%29\n\t"
+      "ds_read2st64_b32 %6, %14 offset0:%30 offset1:%31\n\t"
+      "ds_read2st64_b32 %7, %14 offset0:%32 offset1:%33\n\t"
+      "ds_read_b128 %8, %15 offset:%34\n\t"
+      "ds_read_b128 %9, %15 offset:%35\n\t"
+      "ds_read_b128 %10, %15 offset:%36\n\t"
+      "ds_read_b128 %11, %15 offset:%37\n\t"
+      "ds_read_b128 %12, %16\n\t"
+      "ds_read_b128 %13, %17\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7]),
+        "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3]), "=&v"(x[0][0]), "=&v"(x[0][1])
+      : "v"(wa), "v"(sa), "v"(xa0), "v"(xa1), "i"(8 * (S0 + 0) + 0), "i"(8 * (S0 + 0) + 1), "i"(8 * (S0 + 0) + 2),
+        "i"(8 * (S0 + 0) + 3), "i"(8 * (S0 + 0) + 4), "i"(8 * (S0 + 0) + 5), "i"(8 * (S0 + 0) + 6),
+        "i"(8 * (S0 + 0) + 7), "i"(8 * (S0 + 1) + 0), "i"(8 * (S0 + 1) + 1), "i"(8 * (S0 + 1) + 2),
+        "i"(8 * (S0 + 1) + 3), "i"(8 * (S0 + 1) + 4), "i"(8 * (S0 + 1) + 5), "i"(8 * (S0 + 1) + 6),
+        "i"(8 * (S0 + 1) + 7), "i"(128 * (S0 + 0) + 0), "i"(128 * (S0 + 0) + 16), "i"(128 * (S0 + 1) + 0),
+        "i"(128 * (S0 + 1) + 16)
+      : "memory");
+}
+template <int S0>
+__device__ __forceinline__ void mx_read_nn(unsigned wa, unsigned sa, unsigned xa0, unsigned xa1, u32x2 (&w)[8], u32x4 (&s)[4],
+                                           u32x4 (&x)[2][2]) {
+  asm volatile(
+      "ds_read2st64_b32 %0, %16 offset0:%20 offset1:%21\n\t"
+      "ds_read2st64_b32 %1, %16 offset0:%22 offset1:%23\n\t"
+      "ds_read2st64_b32 %2, %16 offset0:%24 offset1:%25\n\t"
+      "ds_read2st64_b32 %3, %16 offset0:%26 offset1:%27\n\t"
+      "ds_read2st64_b32 %4, %16 offset0:%28 offset1:%29\n\t"
+      "ds_read2st64_b32 %5, %16 offset0:%30 offset1:%31\n\t"
+      "ds_read2st64_b32 %6, %16 offset0:%32 offset1:%33\n\t"
+      "ds_read2st64_b32 %7, %16 offset0:%34 offset1:%35\n\t"
+      "ds_read_b128 %8, %17 offset:%36\n\t"
+      "ds_read_b128 %9, %17 offset:%37\n\t"
+      "ds_read_b128 %10, %17 offset:%38\n\t"
+      "ds_read_b128 %11, %17 offset:%39\n\t"
+      "ds_read_b128 %12, %18\n\t"
+      "ds_read_b128 %13, %19\n\t"
+      "ds_read_b128 %14, %18 offset:4096\n\t"
+      "ds_read_b128 %15, %19 offset:4096\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7]),
+        "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3]), "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]),
+        "=&v"(x[1][1])
+      : "v"(wa), "v"(sa), "v"(xa0), "v"(xa1), "i"(8 * (S0 + 0) + 0), "i"(8 * (S0 + 0) + 1), "i"(8 * (S0 + 0) + 2),
+        "i"(8 * (S0 + 0) + 3), "i"(8 * (S0 + 0) + 4), "i"(8 * (S0 + 0) + 5), "i"(8 * (S0 + 0) + 6),
+        "i"(8 * (S0 + 0) + 7), "i"(8 * (S0 + 1) + 0), "i"(8 * (S0 + 1) + 1), "i"(8 * (S0 + 1) + 2),
+        "i"(8 * (S0 + 1) + 3), "i"(8 * (S0 + 1) + 4), "i"(8 * (S0 + 1) + 5), "i"(8 * (S0 + 1) + 6),
+        "i"(8 * (S0 + 1) + 7), "i"(128 * (S0 + 0) + 0), "i"(128 * (S0 + 0) + 16), "i"(128 * (S0 + 1) + 0),
+        "i"(128 * (S0 + 1) + 16)
+      : "memory");
+}
+
+template <int MT>
+constexpr int mx_nn_lds_bytes(int stages) {
+  return kLdsWaves * (stages * (MT * 4096 + 8192 + 512) > MT * 8192 ? stages * (MT * 4096 + 8192 + 512) : MT * 8192);
+}
+
+template <int MT, int S, typename O>
+__global__ __launch_bounds__(kLdsWaves * 64) void mx_nn_lds_k(const MxArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int kX = MT * 4096, kW = 8192, kStage = kX + kW + 512;
+  constexpr int L = MT * 4 + 8 + 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+  int mb, tile;
+  mx_tile(a, (a.M + 16 * MT - 1) / (16 * MT), (a.cols + 127) >> 7, &mb, &tile);
+  const int k0 = tile * 128, m0 = mb * 16 * MT;
+  const int stages = (a.N + 127) >> 7;
+  const int sb = (int)((int64_t)wave * stages / kLdsWaves), n = (int)((int64_t)(wave + 1) * stages / kLdsWaves) - sb;
+  uint8_t* ring = lds + wave * (S * kStage);
+  const uint8_t* xs[MT * 4];
+#pragma unroll
+  for (int i = 0; i < MT * 4; ++i) {
+    const int r = 4 * i + (lane >> 4), m = min(m0 + r, a.M - 1);
+    xs[i] = reinterpret_cast<const uint8_t*>(a.x + m * a.ld) + sb * 256 + ((l15 ^ (r & 15)) << 4);
+  }
+  const int wrow = ((lane >> 2) & 3) * 8 + (lane >> 4);
+  const uint8_t* wcol = a.codes + (int64_t)tile * 64 + (lane & 3) * 16;
+  const uint8_t* scol = a.scales + tile * 4;
+  const int64_t wld = (int64_t)a.nb * 16;
+  // weight rows behind the end read the last row: the activations there are zeros
+  auto issue = [&](int t) {
+    uint8_t* st = ring + (t % S) * kStage;
+    const int nn = (sb + t) * 128;
+#pragma unroll
+    for (int i = 0; i < MT * 4; ++i) lds_dma16(xs[i] + t * 256, st + i * 1024);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      lds_dma16(wcol + min(nn + wrow + 4 * (j & 1) + 32 * (j >> 1), a.N - 1) * wld, st + kX + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) lds_dma4(scol + (int64_t)min(nn + 64 * j + lane, a.N - 1) * a.nb, st + kX + kW + j * 256);
+  };
+  f32x4 acc[MT][8];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const unsigned turn = 8 * (l15 >> 2) + 9;  // rotates the scale byte of this lane's block to a float's exponent
+  auto use = [&](const u32x2 (&w)[8], const u32x4 (&s)[4], const u32x4 (&x)[MT][2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      union {
+        u16x8 v;
+        unsigned w[4];
+      } row[8], f;  // row[r].w[q]: columns 2 q, 2 q + 1 of weight row r
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const unsigned b = s[2 * h + (r >> 2)][r & 3];
+        row[r].v = mx_fragment(w[4 * h + (r >> 1)][r & 1], __uint_as_float(__builtin_amdgcn_alignbit(b, b, turn) & 0x7f800000u));
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)  // rows 2 q, 2 q + 1 of column c
+          f.w[q] = __builtin_amdgcn_perm(row[2 * q + 1].w[c >> 1], row[2 * q].w[c >> 1], (c & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][c] = mfl::mma16<bf16_t>(__builtin_bit_cast(u16x8, x[i][h]), f.v, acc[i][c]);
+      }
+    }
+  };
+  const unsigned base = mfl::lds_addr(ring);
+  for (int t = 0; t < S - 1 && t < n; ++t) issue(t);
+  for (int t = 0; t < n; ++t) {
+    if (t + S - 1 < n) issue(t + S - 1);
+    const int ahead = n - 1 - t;
+    if (ahead >= S - 1) mx_wait_vm<(S - 1) * L>();
+    else if (S > 2 && ahead == 1) mx_wait_vm<L>();
+    else mx_wait_vm<0>();
+    const unsigned at = base + (t % S) * kStage;
+    const unsigned wa = at + kX + g * 64 + l15 * 4, sa = at + kX + kW + g * 32, xr = at + l15 * 256;
+    u32x2 w[8];
+    u32x4 s[4], x[MT][2];
+    mx_read_nn<0>(wa, sa, xr + ((g ^ l15) << 4), xr + (((4 + g) ^ l15) << 4), w, s, x);
+    use(w, s, x);
+    mx_read_nn<2>(wa, sa, xr + (((8 + g) ^ l15) << 4), xr + (((12 + g) ^ l15) << 4), w, s, x);
+    use(w, s, x);
+  }
+  __syncthreads();  // the rings become the partial tiles
+  constexpr int kTile = MT * 16 * 128;
+  float* part = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float* p = part + wave * kTile + (16 * i + 4 * g + e) * 128 + 8 * l15;
+      reinterpret_cast<float4*>(p)[0] = make_float4(acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(acc[i][4][e], acc[i][5][e], acc[i][6][e], acc[i][7][e]);
+    }
+  __syncthreads();
+  O* y = static_cast<O*>(a.y);
+  for (int t = threadIdx.x; t < kTile; t += kLdsWaves * 64) {
+    const int m = m0 + (t >> 7), k = k0 + (t & 127);
+    if (m >= a.M || k >= a.cols) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kLdsWaves; ++w) sum += part[w * kTile + t];
+    st1<O>(y + (int64_t)m * a.cols + k, sum);
+  }
+}
+
 }  // namespace
 
 hipError_t mx_quantize(int dtype, const void* x, int64_t ld, int64_t rows, int cols, uint8_t* codes, uint8_t* scales,
@@ -475,45 +823,41 @@ namespace {
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 template <typename K>
-hipError_t mx_launch(K kernel, int rows, int tiles, size_t lds, const MxArgs& a, hipStream_t stream) {
-  const int64_t grid = (int64_t)rows * ((tiles + 7) / 8 * 8);
+hipError_t mx_launch(K kernel, int rows, int tiles, int waves, size_t lds, const MxArgs& a, hipStream_t stream) {
+  const int64_t grid = (int64_t)rows * tiles;
   if (grid >= kMxGridMax) return hipErrorInvalidValue;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kMxWaves * 64), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(waves * 64), lds, stream, a);
   return hipGetLastError();
 }
 
+// row blocks whose activations (rows of `bytes`) take at most 2 MB
+int mx_group(int mt, int64_t bytes) {
+  return (int)std::max<int64_t>(1, (2 << 20) / (16 * (mt % kMxLds) * bytes));
+}
+
+bool mx_lds_ok(const uint8_t* scales, int nb) { return nb % 4 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0; }
+
 }  // namespace
 
-// Measured (MI355X, bf16): the one-launch product against decoding the weight (8 us for 4096 x 4096, 18 for 11008 x
-// 4096) plus the tiled GEMM (17 us at least): the larger tiles while they give every CU a workgroup.
-void mx_nt_plan(int M, int N, int nb, int* mt, int* nt) {
-  struct T {
-    int mt, nt;
-  };
-  static const T kOrder[] = {{4, 4}, {2, 4}, {2, 2}, {1, 2}, {1, 1}};
-  const int64_t work = (int64_t)M * N * nb;
-  *mt = *nt = 0;
-  if (M > 128 && work > (int64_t)256 * 4096 * 128) return;
-  for (const T& t : kOrder) {
-    *mt = t.mt;
-    *nt = t.nt;
-    if (16 * t.mt <= M && (int64_t)ceil_div(M, 16 * t.mt) * ceil_div(N, 16 * t.nt) >= 256) return;
-  }
-}
+// Planning.  A variant is a tile, + kMxLds in its rows where the operands go through LDS (rows of whole groups of four
+// blocks); 0 is decoding the weight and the tiled GEMM.  Every variant is priced by its workgroups' rounds over 256 CUs
+// and a round's time, fitted to MI355X measurements (us, bf16 activations):
+//   forward      rows   1     16    32    64    128   333   700   1500       decoded: 128   700   1500  4064
+//   4096 x 4096         4.8   4.9   5.9   7.5   10.5  26    51    100                 31    58    79    134
+//   11008 x 4096        6.9   8.3   9.8   18    27    66    124   256                 49    137   217   376
+//   768 x 2048          3.7   3.7   3.8   3.8   4.3   5.8   11    18                  17    22    26    35
+//   gradient (N -> K)
+//   4096 -> 4096        14    14    14    15    17    34    50    99                  29    60    85    139
+//   11008 -> 4096       33    34    34    35    38    74    113   231                 49    116   215   346
+// (direct, without LDS: forward 4096 x 4096 5.0, 13 at 24 rows, 41 at 100; gradient 19 .. 21 up to 100 rows).
 
-void mx_nn_plan(int M, int N, int nb, int* mt) {
-  const int64_t work = (int64_t)M * N * nb;
-  *mt = M > 128 && work > (int64_t)256 * 4096 * 128 ? 0 : (ceil_div(M, 32) * ceil_div(nb, 4) >= 256 ? 2 : 1);
-}
-
-// The tiled GEMM's 256x256 ping-pong tile (one workgroup a CU) or its 128x128 tile (two a CU), by the rounds that
-// their workgroups need: a 32-deep step of a round takes 1.0 us / 0.62 us (measured at 2032 .. 4064 rows), a split
-// another pass over fp32 partial sums.
-void mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
+// the tiled GEMM's 256 x 256 ping-pong tile (one workgroup a CU) or its 128 x 128 tile (two a CU) by the rounds that their
+// workgroups need: a 32-deep step of a round takes 1.0 / 0.62 us, a split another pass over fp32 partial sums
+double mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
   double best = 1e30;
   *tile = 3;
   *splits = 1;
@@ -533,22 +877,80 @@ void mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
       }
     }
   }
+  return best;
+}
+
+namespace {
+
+// decoding (2.5 bytes an element at the copy rate), and the GEMM of an [M, n] result over k
+double decoded_us(int M, int n, int k, int64_t weight) {
+  int tile, splits;
+  return 5.0 + (double)weight * 0.375e-6 + mx_gemm_plan(M, n, k, &tile, &splits);
+}
+
+}  // namespace
+
+void mx_nt_plan(int M, int N, int nb, bool lds, int* mt, int* nt) {
+  // a round's time is a + b * groups; two or more workgroups a CU (whole = false) fill its rounds evenly
+  static const struct {
+    int mt, nt;
+    double a, b;
+    bool whole;
+  } kTiles[] = {{2, 4, 1.07, 0.217, true}, {2, 2, 0.6, 0.14, true}, {1, 4, 0.2, 0.1625, true}, {1, 2, 0.23, 0.096, false},
+                {1, 1, 0.2, 0.07, false}};
+  const int K = 32 * nb;
+  double best = 1e30;
+  for (const auto& t : kTiles) {
+    if (!lds) break;
+    const double w = (double)ceil_div(M, 16 * t.mt) * ceil_div(N, 16 * t.nt) / 256.0;
+    const double us = 2.5 + (t.a + t.b * (nb / 4)) * std::max(1.0, t.whole ? std::ceil(w) : w);
+    if (us < best) {
+      best = us;
+      *mt = t.mt + kMxLds;
+      *nt = t.nt;
+    }
+  }
+  if (!lds) {  // direct: 250 TFLOP/s in 2 x 4 tiles where they fill the chip
+    const bool wide = M > 16 && (int64_t)ceil_div(M, 32) * ceil_div(N, 64) >= 160;
+    *mt = wide ? 2 : 1;
+    *nt = wide ? 4 : 1;
+    best = 2.5 + 2.0 * M * N * K / 250e6;
+  }
+  if (decoded_us(M, N, K, (int64_t)N * K) < best) *mt = *nt = 0;
+}
+
+void mx_nn_plan(int M, int N, int nb, bool lds, int* mt) {
+  const int K = 32 * nb;
+  lds = lds && N >= 1024 && N % 128 == 0;  // else the direct product is as fast, and activations need no padding
+  const int rows = lds && (int64_t)ceil_div(M, 16) * ceil_div(nb, 4) > 256 ? 2 : 1;
+  const int64_t rounds = (ceil_div(M, 16 * rows) * (int64_t)ceil_div(nb, 4) + 255) / 256;
+  const double us = 2.5 + rounds * (lds ? 1.0 + (rows == 2 ? 0.48 : 0.36) * N / 128 : 0.5 + 0.6 * N / 128);
+  *mt = decoded_us(M, K, N, (int64_t)N * K) < us ? 0 : rows + (lds ? kMxLds : 0);
 }
 
 hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
                  int out_dtype, void* y, hipStream_t stream, int mt, int nt) {
   if (M == 0 || N == 0) return hipSuccess;
   if (out_dtype != kBF16 && out_dtype != kF32) return hipErrorInvalidValue;
-  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, bias, y, M, N, nb, 0, 0};
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, bias, y, M, N, nb, 0, 0, mx_group(mt, 64 * nb)};
+  const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = nt > 0 ? ceil_div(N, 16 * nt) : 0;
+  if (mt > kMxLds && !mx_lds_ok(scales, nb)) return hipErrorInvalidValue;
 #define HYP_MX_NT(MT, NT)                                                                                      \
   if (mt == MT && nt == NT) {                                                                                  \
     const size_t lds = sizeof(float) * kMxWaves * MT * NT * 256;                                               \
-    const int rows = ceil_div(M, 16 * MT), tiles = ceil_div(N, 16 * NT);                                       \
-    return out_dtype == kBF16 ? mx_launch(mx_nt_k<MT, NT, bf16_t>, rows, tiles, lds, a, stream)                \
-                              : mx_launch(mx_nt_k<MT, NT, float>, rows, tiles, lds, a, stream);                \
+    return out_dtype == kBF16 ? mx_launch(mx_nt_k<MT, NT, bf16_t>, rows, tiles, kMxWaves, lds, a, stream)      \
+                              : mx_launch(mx_nt_k<MT, NT, float>, rows, tiles, kMxWaves, lds, a, stream);      \
   }
-  HYP_MX_NT(1, 1) HYP_MX_NT(1, 2) HYP_MX_NT(2, 2) HYP_MX_NT(2, 4) HYP_MX_NT(4, 4)
+#define HYP_MX_NT_LDS(MT, NT)                                                                                  \
+  if (mt == MT + kMxLds && nt == NT) {                                                                         \
+    const size_t lds = mx_nt_lds_bytes<MT, NT>(3);                                                             \
+    return out_dtype == kBF16 ? mx_launch(mx_nt_lds_k<MT, NT, 3, bf16_t>, rows, tiles, kLdsWaves, lds, a, stream) \
+                              : mx_launch(mx_nt_lds_k<MT, NT, 3, float>, rows, tiles, kLdsWaves, lds, a, stream); \
+  }
+  HYP_MX_NT(1, 1) HYP_MX_NT(2, 4)
+  HYP_MX_NT_LDS(1, 1) HYP_MX_NT_LDS(1, 2) HYP_MX_NT_LDS(1, 4) HYP_MX_NT_LDS(2, 2) HYP_MX_NT_LDS(2, 4)
 #undef HYP_MX_NT
+#undef HYP_MX_NT_LDS
   return hipErrorInvalidValue;
 }
 
@@ -556,16 +958,22 @@ hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t*
                  int out_dtype, void* y, hipStream_t stream, int mt) {
   if (M == 0 || cols == 0) return hipSuccess;
   if ((out_dtype != kBF16 && out_dtype != kF32) || ld % 8 != 0) return hipErrorInvalidValue;
-  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld};
-#define HYP_MX_NN(MT)                                                                                          \
-  if (mt == MT) {                                                                                              \
-    const size_t lds = sizeof(float) * kMxWaves * MT * 2048;                                                   \
-    const int rows = ceil_div(M, 16 * MT), tiles = ceil_div(cols, 128);                                        \
-    return out_dtype == kBF16 ? mx_launch(mx_nn_k<MT, bf16_t>, rows, tiles, lds, a, stream)                    \
-                              : mx_launch(mx_nn_k<MT, float>, rows, tiles, lds, a, stream);                    \
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld, mx_group(mt, 2 * ld)};
+  const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = ceil_div(cols, 128);
+  if (mt > kMxLds && (!mx_lds_ok(scales, nb) || ld % 128 != 0)) return hipErrorInvalidValue;
+  if (mt == 1) {
+    const size_t lds = sizeof(float) * kMxWaves * 2048;
+    return out_dtype == kBF16 ? mx_launch(mx_nn_k<bf16_t>, rows, tiles, kMxWaves, lds, a, stream)
+                              : mx_launch(mx_nn_k<float>, rows, tiles, kMxWaves, lds, a, stream);
   }
-  HYP_MX_NN(1) HYP_MX_NN(2)
-#undef HYP_MX_NN
+#define HYP_MX_NN_LDS(MT, S)                                                                                   \
+  if (mt == MT + kMxLds) {                                                                                     \
+    const size_t lds = mx_nn_lds_bytes<MT>(S);                                                                 \
+    return out_dtype == kBF16 ? mx_launch(mx_nn_lds_k<MT, S, bf16_t>, rows, tiles, kLdsWaves, lds, a, stream) \
+                              : mx_launch(mx_nn_lds_k<MT, S, float>, rows, tiles, kLdsWaves, lds, a, stream); \
+  }
+  HYP_MX_NN_LDS(1, 3) HYP_MX_NN_LDS(2, 2)
+#undef HYP_MX_NN_LDS
   return hipErrorInvalidValue;
 }
 

@@ -52,6 +52,8 @@ class MXFP4Tensor:
         self.codes, self.scales, self.shape = codes.contiguous(), scales.contiguous(), shape
         if self.codes.data_ptr() % 16:
             self.codes = self.codes.clone()  # the kernels read 16 bytes at a time
+        if self.scales.data_ptr() % 4:
+            self.scales = self.scales.clone()  # and four scales
 
     @property
     def device(self) -> torch.device:

@@ -85,7 +85,7 @@ def test_strided_activations(M):
     check_linear(96, 40, M, torch.bfloat16, False, view=lambda t: t.t().contiguous().t())
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 100, 160), (33, 300, 96), (70, 72, 384), (200, 264, 1056)])
+@pytest.mark.parametrize("M,N,K", [(1, 100, 160), (33, 300, 96), (70, 72, 384), (200, 264, 1056), (5, 1030, 2048), (40, 128, 128)])
 def test_every_tile_gives_the_same_product(M, N, K):
     C = _native.native()
     g = torch.Generator().manual_seed(M)
@@ -97,10 +97,11 @@ def test_every_tile_gives_the_same_product(M, N, K):
         xd, dd = x.double(), dy.double()
         want = xd @ W.t() + b.double()
         bound = product_bound(xd, W.t(), dtype) + (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * (b.double().abs() + want.abs())
-        for mt, nt in ((0, 0), (1, 1), (1, 2), (2, 2), (2, 4), (4, 4)):
+        lds = [] if w.scales.shape[1] % 4 else [(9, 1), (9, 2), (9, 4), (10, 2), (10, 4)]
+        for mt, nt in [(0, 0), (1, 1), (2, 4)] + lds:
             y = C.mx_linear(x, w.codes, w.scales, b, 16 * mt + nt)
             assert ((y.double() - want).abs() <= bound).all(), (mt, nt)
-        for mt in (0, 1, 2):
+        for mt in [0, 1] + ([9, 10] if lds else []):
             dx = C.mx_linear_dgrad(dy, w.codes, w.scales, K, mt)
             assert ((dx.double() - dd @ W).abs() <= product_bound(dd, W, dtype)).all(), mt
 
@@ -133,6 +134,11 @@ def test_misaligned_codes_are_taken():
     m = MXFP4Tensor(buf[1:].view(8, 32), q.scales, q.shape)
     x = torch.randn(3, 64, device=DEV, dtype=torch.bfloat16)
     assert torch.equal(mxfp4_linear(x, m), mxfp4_linear(x, q))
+    q = quantize_mxfp4(torch.randn(8, 128, device=DEV))
+    buf = torch.empty(q.scales.numel() + 1, dtype=torch.uint8, device=DEV)
+    buf[1:] = q.scales.view(-1)
+    x = torch.randn(3, 128, device=DEV, dtype=torch.bfloat16)
+    assert torch.equal(mxfp4_linear(x, MXFP4Tensor(q.codes, buf[1:].view(8, 4), q.shape)), mxfp4_linear(x, q))
 
 
 @pytest.mark.parametrize("M", [3, 200])
