@@ -189,6 +189,10 @@ void adam8_mt(const at::Tensor& ptrs, const at::Tensor& sizes, const at::Tensor&
               const c10::optional<at::Tensor>& found_inf, int64_t grad_dtype, int64_t param_dtype, bool zero_grad) {
   TORCH_CHECK(sizes.numel() == T && ptrs.numel() == T * (param_dtype == hyp::kF32 ? 6 : 7),
               "adam8_mt: table of 6 (low-precision parameters: 7) x T pointers and T sizes");
+  for (const auto* t : {&lr_t, &inv_scale, &found_inf})
+    TORCH_CHECK(!t->has_value() || !(*t)->defined() || (*t)->device() == ptrs.device(),
+                "adam8_mt: lr, inv_scale and found_inf tensors must be on the table's device");
+  TORCH_CHECK(step_t.device() == ptrs.device(), "adam8_mt: step on another device than the table");
   const at::DeviceGuard guard(ptrs.device());
   HYP_CHECK_HIP(hyp::adam8_multi_tensor((int)grad_dtype, (int)param_dtype, ptrs.data_ptr<int64_t>(),
                                         sizes.data_ptr<int64_t>(), blocks.data_ptr<int>(), (int)blocks.size(0), (int)T,

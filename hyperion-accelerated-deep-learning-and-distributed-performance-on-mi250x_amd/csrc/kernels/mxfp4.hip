@@ -834,9 +834,10 @@ hipError_t mx_launch(K kernel, int rows, int tiles, int waves, size_t lds, const
   return hipGetLastError();
 }
 
-// row blocks whose activations (rows of `bytes`) take at most 2 MB
-int mx_group(int mt, int64_t bytes) {
-  return (int)std::max<int64_t>(1, (2 << 20) / (16 * (mt % kMxLds) * bytes));
+// row blocks (of M rows) whose activations, rows of `bytes`, take at most 2 MB
+int mx_group(int M, int mt, int64_t bytes) {
+  const int rows = 16 * (mt % kMxLds);
+  return rows == 0 ? 1 : (int)std::min<int64_t>(ceil_div(M, rows), std::max<int64_t>(1, (2 << 20) / (rows * bytes)));
 }
 
 bool mx_lds_ok(const uint8_t* scales, int nb) { return nb % 4 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0; }
@@ -932,8 +933,9 @@ hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int
                  int out_dtype, void* y, hipStream_t stream, int mt, int nt) {
   if (M == 0 || N == 0) return hipSuccess;
   if (out_dtype != kBF16 && out_dtype != kF32) return hipErrorInvalidValue;
-  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, bias, y, M, N, nb, 0, 0, mx_group(mt, 64 * nb)};
-  const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = nt > 0 ? ceil_div(N, 16 * nt) : 0;
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, bias, y, M, N, nb, 0, 0, mx_group(M, mt, (int64_t)64 * nb)};
+  if (mt % kMxLds == 0 || nt <= 0) return hipErrorInvalidValue;
+  const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = ceil_div(N, 16 * nt);
   if (mt > kMxLds && !mx_lds_ok(scales, nb)) return hipErrorInvalidValue;
 #define HYP_MX_NT(MT, NT)                                                                                      \
   if (mt == MT && nt == NT) {                                                                                  \
@@ -958,7 +960,8 @@ hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t*
                  int out_dtype, void* y, hipStream_t stream, int mt) {
   if (M == 0 || cols == 0) return hipSuccess;
   if ((out_dtype != kBF16 && out_dtype != kF32) || ld % 8 != 0) return hipErrorInvalidValue;
-  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld, mx_group(mt, 2 * ld)};
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld, mx_group(M, mt, 2 * ld)};
+  if (mt % kMxLds == 0) return hipErrorInvalidValue;
   const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = ceil_div(cols, 128);
   if (mt > kMxLds && (!mx_lds_ok(scales, nb) || ld % 128 != 0)) return hipErrorInvalidValue;
   if (mt == 1) {

@@ -28,16 +28,16 @@ from typing import Dict, Iterable, List, Optional
 import torch
 import torch.nn as nn
 
-from ..ops.cross_entropy import LinearCrossEntropy
 from ..ops.dropout import dropout
-from ..ops.linear import linear
+from ..ops.linear import Linear, linear
 from ..ops.lora import lora_linear
 from ..ops.mxfp4 import MXFP4Linear, MXFP4Tensor
 
 
 class LoRALinear(nn.Module):
-    def __init__(self, base: nn.Linear, r: int = 16, alpha: float = 32.0, dropout: float = 0.05,
-                 adapter: str = "default"):
+    def __init__(self, base: nn.Module, r: int = 16, alpha: float = 32.0, dropout: float = 0.05,
+                 adapter: str = "default", dtype: Optional[torch.dtype] = None):
+        """``base``: an ``nn.Linear`` or an ``MXFP4Linear``, whose adapter takes ``dtype`` (default: torch's)."""
         super().__init__()
         self.base_layer = base
         self.in_features, self.out_features = base.in_features, base.out_features
@@ -45,16 +45,16 @@ class LoRALinear(nn.Module):
         self.lora_alpha = alpha
         self.scaling = {adapter: alpha / r}
         self.adapter = adapter
-        dev, dt = base.weight.device, base.weight.dtype
+        dev = base.weight.device
+        dt = (dtype or torch.get_default_dtype()) if isinstance(base, MXFP4Linear) else base.weight.dtype
         self.lora_A = nn.ModuleDict({adapter: nn.Linear(base.in_features, r, bias=False, device=dev, dtype=dt)})
         self.lora_B = nn.ModuleDict({adapter: nn.Linear(r, base.out_features, bias=False, device=dev, dtype=dt)})
         self.lora_dropout = nn.ModuleDict({adapter: nn.Dropout(dropout) if dropout > 0 else nn.Identity()})
         self.p = dropout
         nn.init.kaiming_uniform_(self.lora_A[adapter].weight, a=math.sqrt(5))
         nn.init.zeros_(self.lora_B[adapter].weight)
-        base.weight.requires_grad_(False)
-        if base.bias is not None:
-            base.bias.requires_grad_(False)
+        for p in base.parameters():
+            p.requires_grad_(False)
 
     @property
     def weight(self) -> torch.Tensor:  # code that reads q_proj.weight keeps working
@@ -89,23 +89,24 @@ def apply_lora(model: nn.Module, r: int = 16, alpha: float = 32.0, dropout: floa
     targets = set(target_modules)
     for p in model.parameters():
         p.requires_grad_(False)
+    dtype = next((p.dtype for p in model.parameters() if p.is_floating_point()), None)
     for name, mod in list(model.named_modules()):
         for cname, child in list(mod.named_children()):
-            if cname in targets and isinstance(child, nn.Linear) and not isinstance(child, LoRALinear):
-                setattr(mod, cname, LoRALinear(child, r, alpha, dropout, adapter))
+            if cname in targets and isinstance(child, (nn.Linear, MXFP4Linear)) and not isinstance(mod, LoRALinear):
+                setattr(mod, cname, LoRALinear(child, r, alpha, dropout, adapter, dtype))
     model.peft_config = {adapter: lora_config_dict(r, alpha, dropout, sorted(targets))}
     return quantize_base(model) if base_format == "mxfp4" else model
 
 
 def quantize_base(model: nn.Module) -> nn.Module:
-    """Hold every frozen linear layer (a LoRA layer's base among them) in 4 bits, in place.  LM heads
-    (``LinearCrossEntropy``) and layers with trainable weights stay as they are."""
+    """Hold every frozen plain linear layer (``nn.Linear`` or ``ops.linear.Linear``; a LoRA layer's base among
+    them) in 4 bits, in place.  Subclasses that do more (LM heads, fused activations) and layers with
+    trainable weights stay as they are."""
     adapters = {id(m) for lora in model.modules() if isinstance(lora, LoRALinear)
                 for d in (lora.lora_A, lora.lora_B) for m in d.values()}
     for mod in list(model.modules()):
         for cname, child in list(mod.named_children()):
-            if (isinstance(child, nn.Linear) and not isinstance(child, LinearCrossEntropy)
-                    and not child.weight.requires_grad and id(child) not in adapters):
+            if type(child) in (nn.Linear, Linear) and not child.weight.requires_grad and id(child) not in adapters:
                 setattr(mod, cname, MXFP4Linear.from_linear(child))
     return model
 

@@ -85,13 +85,14 @@ def _decode_reference(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor
     q = torch.stack([codes & 15, codes >> 4], dim=-1).view(codes.shape[0], scales.shape[1], BLOCK)
     s = torch.exp2(scales.double() - 127.0).float()
     s = torch.where(scales == 255, torch.full_like(s, math.nan), s)
-    return (table[q.long()] * s[..., None]).view(codes.shape[0], -1)
+    return (table[q.long()] * s[..., None]).view(codes.shape[0], 2 * codes.shape[1])
 
 
 def _encode_reference(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """PyTorch oracle of mx_quantize over [R, K]."""
     R, K = x.shape
-    x = F.pad(x.float(), (0, -K % BLOCK)).view(R, -1, BLOCK)
+    nb = -(-K // BLOCK)
+    x = F.pad(x.float(), (0, -K % BLOCK)).view(R, nb, BLOCK)
     amax = x.abs().amax(dim=2, keepdim=True)
     bad = ~torch.isfinite(amax)
     e = (torch.frexp(torch.where(bad, torch.ones_like(amax), amax))[1] - 3).clamp(min=-127)
@@ -100,7 +101,7 @@ def _encode_reference(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
     a = (torch.round(a / step) * step).clamp(max=6.0)
     code = torch.where(a < 2, a * 2, torch.where(a < 4, a + 2, a / 2 + 4)).nan_to_num(0.0).to(torch.uint8)
-    code = (code | (torch.signbit(x).to(torch.uint8) << 3)).view(R, -1, 2)
+    code = (code | (torch.signbit(x).to(torch.uint8) << 3)).view(R, 16 * nb, 2)
     scale = torch.where(bad, torch.full_like(e, 255), e + 127).to(torch.uint8)
     return code[..., 0] | (code[..., 1] << 4), scale[..., 0]
 
@@ -168,7 +169,7 @@ class _MXLinearFn(torch.autograd.Function):
             else:
                 dx = (dy.float() @ w._rows(torch.float32, K)).to(dy.dtype)
         if ctx.bdtype is not None and ctx.needs_input_grad[1]:
-            db = bias_grad(dy.reshape(-1, N).contiguous(), ctx.bdtype)
+            db = bias_grad(dy.reshape(math.prod(dy.shape[:-1]), N).contiguous(), ctx.bdtype)
         return dx, db, None
 
 
@@ -214,7 +215,8 @@ class MXFP4Linear(nn.Module):
     def weight(self) -> MXFP4Tensor:
         return MXFP4Tensor(self.weight_codes, self.weight_scales, (self.out_features, self.in_features))
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, link=None, blink=None) -> torch.Tensor:
+        """``link`` / ``blink``: the gradient links of ``ops.linear.Linear``, which stay unarmed here."""
         return mxfp4_linear(x, self.weight, self.bias)
 
     def extra_repr(self) -> str:

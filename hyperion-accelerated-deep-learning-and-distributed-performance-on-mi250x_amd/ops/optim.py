@@ -146,6 +146,7 @@ class FusedAdam(torch.optim.Optimizer):
             st["exp_avg_sq_q"] = torch.zeros(n, dtype=torch.uint8, device=p.device)
             st["exp_avg_scale"] = torch.zeros(nb, dtype=torch.float32, device=p.device)
             st["exp_avg_sq_scale"] = torch.zeros(nb, dtype=torch.float32, device=p.device)
+            st["channels_last"] = _channels_last(p)  # the order of the blocks
             if p.dtype != torch.float32:
                 st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format).clone()
         if not st:
@@ -258,7 +259,7 @@ class FusedAdam(torch.optim.Optimizer):
     def _launch8(self, gi, tab, gdt, pdt, inv_scale) -> None:
         group = self.param_groups[gi]
         lr = group["lr"]
-        lr_t = lr if isinstance(lr, torch.Tensor) else None
+        lr_t = lr if isinstance(lr, torch.Tensor) and lr.is_cuda else None
         b1, b2 = group["betas"]
         _native.count("adam8")
         _native.native().adam8_mt(
@@ -270,9 +271,15 @@ class FusedAdam(torch.optim.Optimizer):
         """One partition (a parameter dtype and a gradient dtype) with 8-bit moments; the launch, or None where the
         reference path ran."""
         pdt, gdt = ps[0].dtype, gs[0].dtype
+        for p, st in zip(ps, sts):  # the kernels trust what the state says
+            if (st["exp_avg_q"].numel() != p.numel() or st["exp_avg_q"].device != p.device
+                    or st["channels_last"] != _channels_last(p)):
+                raise ValueError(f"FusedAdam(state_bits=8): a parameter (now {tuple(p.shape)}, strides {p.stride()}, on "
+                                 f"{p.device}) changed its size, memory format or device after its first step")
         tab = None
         if native and pdt in _native.DTYPE_CODE and gdt in _native.DTYPE_CODE and all(
-                _dense(p) and _dense(g) and _same_layout(p, g) for p, g in zip(ps, gs)):
+                p.device == self._step_t.device and _dense(p) and _dense(g) and _same_layout(p, g)
+                and (pdt == torch.float32 or _same_layout(p, st["master"])) for p, g, st in zip(ps, gs, sts)):
             groups = [ps, gs] + [[s[k] for s in sts] for k in _STATE8]
             if pdt != torch.float32:
                 groups.append([s["master"] for s in sts])
@@ -405,6 +412,9 @@ class FusedAdam(torch.optim.Optimizer):
             if "exp_avg_q" in st:
                 raise ValueError("FusedAdam(state_bits=32): the saved state has 8-bit moments (state_bits=8)")
             return
+        if bool(st.get("channels_last", False)) != _channels_last(p):
+            raise ValueError(f"FusedAdam(state_bits=8): the saved moments of a {tuple(p.shape)} parameter are coded in "
+                             f"another memory format's order than the parameter's")
         n, nb = p.numel(), -(-p.numel() // STATE_BLOCK)
         want = {"exp_avg_q": (torch.int8, n), "exp_avg_sq_q": (torch.uint8, n),
                 "exp_avg_scale": (torch.float32, nb), "exp_avg_sq_scale": (torch.float32, nb)}
@@ -433,8 +443,10 @@ class FusedAdam(torch.optim.Optimizer):
             for k, t in state_dict["state"].get(i, {}).items():
                 if k in _STATE8:
                     self.state[p][k] = t.detach().to(p.device).reshape(-1).clone()
+                    self.state[p]["channels_last"] = _channels_last(p)
                 elif k in ("exp_avg", "exp_avg_sq", "master"):
-                    self.state[p][k] = t.detach().to(p.device, torch.float32).clone()
+                    # (in the parameter's layout, which the kernels take them to have)
+                    self.state[p][k] = torch.empty_like(p, dtype=torch.float32).copy_(t.detach().view(p.shape))
         self._step_t = None
         self._plan8 = self._values8 = None
         # the table cache is kept: tables a captured graph uses stay pinned; new state tensors

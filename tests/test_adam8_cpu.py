@@ -157,3 +157,36 @@ def test_refusals():
         bad["state"][0][key] = value
         with pytest.raises(ValueError, match=key):
             FusedAdam([p], state_bits=8).load_state_dict(bad)
+
+
+def test_memory_format_changes():
+    torch.manual_seed(2)
+    w = torch.randn(5, 7, 3, 3)
+
+    def stepped(fmt, bits, dtype=torch.float32):
+        p = torch.nn.Parameter(w.to(dtype, memory_format=fmt))
+        opt = FusedAdamW([p], state_bits=bits)
+        p.grad = torch.ones_like(p)
+        opt.step()
+        return p, opt
+
+    p, opt = stepped(torch.channels_last, 8)
+    other = torch.nn.Parameter(w.clone())
+    with pytest.raises(ValueError, match="memory format"):
+        FusedAdamW([other], state_bits=8).load_state_dict(opt.state_dict())
+    same = torch.nn.Parameter(w.to(memory_format=torch.channels_last))
+    FusedAdamW([same], state_bits=8).load_state_dict(opt.state_dict())
+    p.data = p.data.contiguous()
+    p.grad = torch.ones(5, 7, 3, 3)
+    with pytest.raises(ValueError, match="memory format"):
+        opt.step()
+    p.data, p.grad = torch.randn(9), torch.randn(9)
+    with pytest.raises(ValueError, match="size"):
+        opt.step()
+    # 32 bits: the moments and masters take the parameter's layout, whatever the saved one
+    p, opt = stepped(torch.channels_last, 32, torch.bfloat16)
+    q = torch.nn.Parameter(w.bfloat16())
+    o2 = FusedAdamW([q])
+    o2.load_state_dict(opt.state_dict())
+    for k in ("exp_avg", "exp_avg_sq", "master"):
+        assert o2.state[q][k].stride() == q.stride() and torch.equal(o2.state[q][k], opt.state[p][k])

@@ -191,3 +191,16 @@ def test_steps_without_changes_do_not_walk_the_tensors(monkeypatch):
     monkeypatch.setattr(opt, "_step8", None)
     monkeypatch.setattr(opt._tables, "get", None)
     opt.step(), opt.moment_vectors()
+
+
+def test_learning_rates_as_tensors():
+    grads = [torch.randn(500, device="cuda") for _ in range(3)]
+    results = []
+    for lr in (0.01, torch.tensor(0.01), torch.tensor(0.01, device="cuda")):
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 500, device="cuda"))
+        opt = FusedAdamW([p], lr=lr, state_bits=8)
+        for g in grads:
+            p.grad = g
+            opt.step()
+        results.append(p.detach().clone())
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])

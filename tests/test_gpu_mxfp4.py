@@ -177,3 +177,15 @@ def test_kernels_are_reached():
     x = torch.randn(4, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
     mxfp4_linear(x, w).sum().backward()
     assert _native.counters() == {"mxfp4_linear": 1, "mxfp4_dgrad": 1}
+
+
+@pytest.mark.parametrize("M,N,K", [(0, 4, 40), (3, 0, 40), (3, 4, 0), (0, 0, 0)])
+def test_empty_sizes(M, N, K):
+    w = quantize_mxfp4(torch.randn(N, K, device="cuda"))
+    assert w.dequantize().shape == (N, K)
+    x, b = torch.randn(M, K, device="cuda", requires_grad=True), torch.randn(N, device="cuda", requires_grad=True)
+    y = mxfp4_linear(x, w, b)
+    assert torch.equal(y, b.detach().expand(M, N))  # sums over nothing
+    dx, db = torch.autograd.grad(y.sum(), [x, b])
+    assert dx.shape == x.shape and (N or not dx.any())
+    assert torch.equal(db, torch.full_like(b, M))

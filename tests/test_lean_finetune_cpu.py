@@ -47,6 +47,26 @@ def test_dropout_and_refusals():
     assert dequantized(m) is not m
 
 
+def test_quantised_first_and_other_models():
+    m = LlamaForCausalLM(LlamaConfig.tiny(num_key_value_heads=1)).bfloat16()
+    for p in m.parameters():
+        p.requires_grad_(False)
+    apply_lora(quantize_base(m), r=4)
+    layers = [x for x in m.modules() if isinstance(x, LoRALinear)]
+    assert len(layers) == 8 and all(isinstance(x.base_layer, MXFP4Linear) for x in layers)
+    assert all(x.lora_A["default"].weight.dtype == torch.bfloat16 for x in layers)
+    from hyperion.models.transformer import create_custom_transformer
+
+    torch.manual_seed(0)
+    t = create_custom_transformer().eval()
+    for p in t.parameters():
+        p.requires_grad_(False)
+    x = torch.randn(2, 5, 512)
+    before = t(x)
+    n = sum(isinstance(c, MXFP4Linear) for c in quantize_base(t).modules())
+    assert n > 0 and t(x).shape == before.shape and torch.isfinite(t(x)).all()
+
+
 def test_trainer_with_a_4_bit_base(tmp_path):
     from hyperion.train.distributed import train_llama_fsdp
     from test_trainers_cpu import _opts

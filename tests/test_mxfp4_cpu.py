@@ -87,6 +87,18 @@ def test_layer_state_dict_and_casts():
         assert mxfp4_linear(x, fresh.weight).dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize("M,N,K", [(0, 4, 40), (3, 0, 40), (3, 4, 0), (0, 0, 0)])
+def test_empty_sizes(M, N, K):
+    w = quantize_mxfp4(torch.randn(N, K, device="cpu"))
+    assert w.dequantize().shape == (N, K)
+    x, b = torch.randn(M, K, device="cpu", requires_grad=True), torch.randn(N, device="cpu", requires_grad=True)
+    y = mxfp4_linear(x, w, b)
+    assert torch.equal(y, b.detach().expand(M, N))  # sums over nothing
+    dx, db = torch.autograd.grad(y.sum(), [x, b])
+    assert dx.shape == x.shape and (N or not dx.any())
+    assert torch.equal(db, torch.full_like(b, M))
+
+
 def test_refusals():
     q = quantize_mxfp4(torch.randn(4, 40))
     x = torch.randn(2, 40)
