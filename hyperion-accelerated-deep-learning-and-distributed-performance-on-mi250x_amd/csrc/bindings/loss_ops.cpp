@@ -60,9 +60,9 @@ LogitRows logit_rows(const at::Tensor& z, const at::Tensor& target, const char* 
   return r;
 }
 
-// (logprobs [...], entropy [...], stats [rows, 3], top logprobs [..., k], top ids [..., k])
+// (logprobs [...], entropy [...], stats [rows, 3] or none, top logprobs [..., k], top ids [..., k]; none without k)
 std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& z, const at::Tensor& target, int64_t k, int64_t ignore_index,
-                                           double inv_t) {
+                                           double inv_t, bool keep_stats) {
   const LogitRows r = logit_rows(z, target, "token_logprobs_fwd");
   TORCH_CHECK(k >= 0 && k <= hyp::kTokenTopMax && k <= r.V, "token_logprobs_fwd: k must be in [0, min(V, ",
               hyp::kTokenTopMax, ")]");
@@ -70,14 +70,20 @@ std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& z, const at::Tensor
   const at::DeviceGuard guard(z.device());
   auto fopt = z.options().dtype(at::kFloat);
   const auto lead = z.sizes().slice(0, z.dim() - 1);
-  auto topk = lead.vec();
-  topk.push_back(k);
-  auto lp = at::empty(lead, fopt), ent = at::empty(lead, fopt), stats = at::empty({r.rows, 3}, fopt);
-  auto tl = at::empty(topk, fopt), ti = at::empty(topk, z.options().dtype(at::kLong));
+  auto lp = at::empty(lead, fopt), ent = at::empty(lead, fopt);
+  at::Tensor stats, tl, ti;  // (a small call is the host's time: nothing is allocated that nobody reads)
+  if (keep_stats) stats = at::empty({r.rows, 3}, fopt);
+  if (k > 0) {
+    auto topk = lead.vec();
+    topk.push_back(k);
+    tl = at::empty(topk, fopt);
+    ti = at::empty(topk, z.options().dtype(at::kLong));
+  }
   HYP_CHECK_HIP(hyp::token_logprobs_fwd(dtype_code(z), z.data_ptr(), r.s0, r.s1, r.inner, r.rows, r.V,
                                         target.data_ptr<int64_t>(), ignore_index, (float)inv_t, lp.data_ptr<float>(),
-                                        ent.data_ptr<float>(), stats.data_ptr<float>(), (int)k, tl.data_ptr<float>(),
-                                        ti.data_ptr<int64_t>(), cur_stream()));
+                                        ent.data_ptr<float>(), keep_stats ? stats.data_ptr<float>() : nullptr, (int)k,
+                                        k > 0 ? tl.data_ptr<float>() : nullptr, k > 0 ? ti.data_ptr<int64_t>() : nullptr,
+                                        cur_stream()));
   return {lp, ent, stats, tl, ti};
 }
 
@@ -190,7 +196,7 @@ void register_loss_ops(pybind11::module& m) {
   m.def("embedding_fwd", &embedding_fwd, "token embedding gather");
   m.def("token_logprobs_fwd", &token_logprobs_fwd, "log probability of each row's target, entropy, top-k alternatives",
         pybind11::arg("logits"), pybind11::arg("target"), pybind11::arg("k"), pybind11::arg("ignore_index"),
-        pybind11::arg("inv_t"));
+        pybind11::arg("inv_t"), pybind11::arg("keep_stats"));
   m.def("token_logprobs_bwd", &token_logprobs_bwd, "gradient of token_logprobs_fwd's log probabilities and entropies",
         pybind11::arg("logits"), pybind11::arg("target"), pybind11::arg("stats"), pybind11::arg("ignore_index"),
         pybind11::arg("inv_t"), pybind11::arg("dlogp"), pybind11::arg("dent"));

@@ -140,7 +140,7 @@ hipError_t cross_entropy_fwd_bwd(int dtype, void* logits, int64_t rows, int V, i
 namespace hyp {
 // ---- token_logprobs.hip ------------------------------------------------------------------------
 // Rows of V logits with unit element stride: row r at (r / inner) * s0 + (r % inner) * s1 elements.
-// stats [rows, 3] is what the backward needs; top_* [rows, k].  dlogp / dent may be null (zeros); dz is
+// stats [rows, 3] is what the backward needs (null: none comes); top_* [rows, k].  dlogp / dent may be null (zeros); dz is
 // contiguous [rows, V].  A launch holds fewer than kTokenRowsMax workgroups of 256 threads.
 constexpr int kTokenTopMax = 32;
 constexpr int64_t kTokenRowsMax = int64_t(1) << 24;

@@ -139,7 +139,7 @@ struct LpArgs {
   const int64_t* target;
   int64_t ignore;
   float c, inv_t;
-  float *logp, *ent, *stats;  // stats [rows, 3]: m, log2 s, H
+  float *logp, *ent, *stats;  // stats [rows, 3]: m, log2 s, H; null without a backward to come
   int k;
   float* top_lp;
   int64_t* top_id;
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
     if (tid == 0) {
       a.logp[row] = 0.f;
       a.ent[row] = 0.f;
-      a.stats[3 * row] = a.stats[3 * row + 1] = a.stats[3 * row + 2] = 0.f;
+      if (a.stats) a.stats[3 * row] = a.stats[3 * row + 1] = a.stats[3 * row + 2] = 0.f;
     }
     if (TOP && tid < a.k) {
       a.top_lp[row * a.k + tid] = 0.f;
@@ -277,9 +277,11 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
     if (h < 0.f) h = 0.f;  // rounding, in a row of one token
     a.logp[row] = lp;
     a.ent[row] = h;
-    a.stats[3 * row] = m;
-    a.stats[3 * row + 1] = ls;
-    a.stats[3 * row + 2] = h;
+    if (a.stats) {
+      a.stats[3 * row] = m;
+      a.stats[3 * row + 1] = ls;
+      a.stats[3 * row + 2] = h;
+    }
   }
   if (!TOP) return;
   auto write = [&](int at, uint64_t key) {

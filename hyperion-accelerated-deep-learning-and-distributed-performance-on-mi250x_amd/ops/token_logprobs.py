@@ -79,19 +79,22 @@ def _reference_bwd(z, target, stats, ignore_index, inv_t, dlogp, dent):
 
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, target, k, ignore_index, inv_t):
+    def forward(ctx, logits, target, k, ignore_index, inv_t, needs_grad):
         native = _native.use_native(logits, op="token_logprobs")
         if native:
             _native.count("token_logprobs")
-            lp, h, stats, tl, ti = _native.native().token_logprobs_fwd(logits, target, k, ignore_index, inv_t)
+            lp, h, stats, tl, ti = _native.native().token_logprobs_fwd(logits, target, k, ignore_index, inv_t,
+                                                                             needs_grad)
         else:
             rows = logits.reshape(-1, logits.shape[-1])
             lp, h, stats, tl, ti = _reference_fwd(rows, target.reshape(-1), k, ignore_index, inv_t)
             lead = logits.shape[:-1]
-            lp, h, tl, ti = lp.view(lead), h.view(lead), tl.view(*lead, k), ti.view(*lead, k)
+            lp, h = lp.view(lead), h.view(lead)
+            tl, ti = (tl.view(*lead, k), ti.view(*lead, k)) if k else (None, None)
         ctx.save_for_backward(logits, target, stats)
         ctx.cfg = (ignore_index, inv_t, native)
-        ctx.mark_non_differentiable(tl, ti)
+        if k:
+            ctx.mark_non_differentiable(tl, ti)
         ctx.set_materialize_grads(False)
         return lp, h, tl, ti
 
@@ -101,7 +104,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
         logits, target, stats = ctx.saved_tensors
         ignore_index, inv_t, native = ctx.cfg
         if dlogp is None and dent is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         dlogp = None if dlogp is None else dlogp.float().contiguous().view(-1)
         dent = None if dent is None else dent.float().contiguous().view(-1)
         if native:
@@ -109,7 +112,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
         else:
             dz = _reference_bwd(logits.reshape(-1, logits.shape[-1]), target.reshape(-1), stats, ignore_index, inv_t,
                                 dlogp, dent).view(logits.shape)
-        return dz, None, None, None, None
+        return dz, None, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, ignore_index: int = -100,
@@ -141,6 +144,6 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, i
         if logits.dim() > 3:
             out = token_logprobs(logits.view(-1, V), target.reshape(-1), top_k, ignore_index, temperature)
             return TokenLogprobs(*(None if t is None else t.view(*target.shape, *t.shape[1:]) for t in out))
-    args = (logits, target.long().contiguous(), int(top_k), int(ignore_index), 1.0 / float(temperature))
-    lp, h, tl, ti = _native.apply_fn(_TokenLogprobsFn, *args, needs_grad=logits.requires_grad)
-    return TokenLogprobs(lp, h, tl if top_k else None, ti if top_k else None)
+    needs_grad = logits.requires_grad and torch.is_grad_enabled()
+    return TokenLogprobs(*_native.apply_fn(_TokenLogprobsFn, logits, target.long().contiguous(), int(top_k),
+                                           int(ignore_index), 1.0 / float(temperature), needs_grad, needs_grad=needs_grad))
