@@ -134,13 +134,19 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& codes, const at::Ten
   const at::Tensor xp = pieces(x, 32 * nb);
   const auto dt = P == 1 ? at::kBFloat16 : at::kFloat;
   int mt, nt;
-  hyp::mx_nt_plan((int)(P * M), (int)N, (int)nb, lds_ok(scales), &mt, &nt);
+  hyp::mx_nt_plan((int)M, (int)N, (int)nb, (int)P, lds_ok(scales), &mt, &nt);
   if (tile >= 0) mt = (int)tile / 16, nt = (int)tile % 16;
   at::Tensor y;
+  if (mt > hyp::kMxBig) {
+    y = at::empty({M, N}, x.options());
+    HYP_CHECK_HIP(hyp::mx_nt(xp.data_ptr(), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), (int)M, (int)N, (int)nb, b,
+                             dtype_code(y), y.data_ptr(), cur_stream(), mt, nt, (int)P));
+    return y;
+  }
   if (mt > 0) {
     y = at::empty({P * M, N}, xp.options().dtype(dt));
     HYP_CHECK_HIP(hyp::mx_nt(xp.data_ptr(), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), (int)(P * M), (int)N,
-                             (int)nb, P == 1 ? b : nullptr, dtype_code(dt), y.data_ptr(), cur_stream(), mt, nt));
+                             (int)nb, P == 1 ? b : nullptr, dtype_code(dt), y.data_ptr(), cur_stream(), mt, nt, 1));
   } else {
     const int64_t Np = (N + 7) / 8 * 8;
     const bool direct = P == 1 && (b == nullptr || Np == N);  // the epilogue's bias has as many elements as columns

@@ -169,16 +169,18 @@ hipError_t mx_join(int dtype, const float* part, int pieces, int64_t rows, int c
                    void* y, hipStream_t stream);
 // y [M, N] (bf16 / fp32) = x [M, 32 nb] (bf16) times the transpose of the 4-bit weight [N, 32 nb] (+ bias), in tiles
 // of 16 mt x 16 nt: 1x1 or 2x4, or through LDS (mt + kMxLds; nb % 4 == 0 and 4-byte aligned scales) 1x1 1x2 1x4 2x2 2x4
-constexpr int kMxLds = 8;
+// or, with that, 32 MI x 128 (mt = kMxBig + MI, MI 2 or 4, nt = 8), which also takes x as pieces [pieces, M, 32 nb] whose sum
+// the activations are, and gives fp16
+constexpr int kMxLds = 8, kMxBig = 16;
 hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
-                 int out_dtype, void* y, hipStream_t stream, int mt, int nt);
+                 int out_dtype, void* y, hipStream_t stream, int mt, int nt, int pieces);
 // y [M, cols] (bf16 / fp32) = x [M, N] (bf16; rows of stride ld, zeros from N to it) times the 4-bit weight [N, 32 nb], in
 // tiles of 16 mt x 128: mt 1 (ld % 8 == 0), or through LDS (mt + kMxLds; also ld % 128 == 0) 1 or 2
 hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, int cols,
                  int out_dtype, void* y, hipStream_t stream, int mt);
 // the tile of mx_nt / mx_nn for a product, 0 where decoding the weight and the tiled GEMM are faster (lds: the weight
 // allows the products through LDS); the tiled GEMM's (tile, splits) for it and their time in us
-void mx_nt_plan(int M, int N, int nb, bool lds, int* mt, int* nt);
+void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt);
 void mx_nn_plan(int M, int N, int nb, bool lds, int* mt);
 double mx_gemm_plan(int M, int N, int K, int* tile, int* splits);
 }  // namespace hyp

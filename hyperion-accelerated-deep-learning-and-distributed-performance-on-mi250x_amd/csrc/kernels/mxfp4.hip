@@ -186,6 +186,7 @@ struct MxArgs {
   int cols;      // NN: columns of y (K of the weight)
   int64_t ld;    // NN: row stride of x
   int group;     // row blocks of a group (mx_tile)
+  int pieces;    // 128-column tiles: x is [pieces, M, 32 nb], their sum the activations
 };
 
 // workgroup -> (row block, weight tile): every XCD takes a contiguous piece of the order row group, weight tile, row
@@ -484,6 +485,166 @@ __global__ __launch_bounds__(kLdsWaves * 64) void mx_nt_lds_k(const MxArgs a) {
     for (int w = 0; w < kLdsWaves; ++w) sum += part[w * kTile + t];
     if (a.bias) sum += a.bias[c];
     st1<O>(y + (int64_t)m * a.N + c, sum);
+  }
+}
+
+// ---- the same product in 128-column tiles -----------------------------------------------------------------
+// For more rows: 8 waves share a ring of stages (one barrier a stage) over 32 MI rows and 128 columns, so that a
+// decoded fragment meets MI fragments of activations.  Waves 4 h + 2 i + j own the i-th half of the rows and the j-th of
+// the columns for half h of every block's elements: two waves a SIMD (one alone issues at half rate), whose
+// sums meet in LDS.  4064 x 11008 x 4096 in 368 us (1.0 PFLOP/s, the tiled GEMM's rate without a decoded weight),
+// 512 x 4096 x 4096 in 25 us against 36 in 32-row tiles.  Halves a barrier apart (one multiplies while the other
+// reads) were slower, 37.6 against 34.6 us at 512 rows, and so was every wave bringing its own scales (42 against 36 us at
+// 700 rows in 64-row tiles).  The images are those above.  x holds P pieces [M, 32 nb] whose sum the activations are: the
+// reduction runs over the weight once for each, the smallest first, into the same fp32 sums.
+constexpr int kBigStages = 3, kBigCols = 128;
+
+__device__ __forceinline__ void st4(float* y, const float (&v)[4]) { *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void st4(bf16_t* y, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+__device__ __forceinline__ void st4(f16_t* y, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(y) = make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
+}
+
+// LDS-DMA as asm (it has no result): with the builtin in flight the compiler waits for the whole ring before an LDS read,
+// and here it is to schedule the fragment reads among the matrix instructions.
+__device__ __forceinline__ void big_dma16(const void* src, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void big_dma4(const void* src, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
+}
+template <typename V>
+__device__ __forceinline__ V lds_at(unsigned addr) {
+  return *(const __attribute__((address_space(3))) V*)addr;
+}
+
+template <int MI>
+constexpr int mx_nt_big_bytes() {
+  return kBigStages * (MI * 8192 + 8192 + 512);
+}
+
+template <int MI, typename O>
+__global__ __launch_bounds__(512) void mx_nt_big_k(const MxArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int kX = MI * 8192, kW = 8192, kStage = kX + kW + 512, S = kBigStages;
+  constexpr int L = MI + 1;  // DMA instructions of a wave and stage; waves 0 and 1 also bring the scales
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+  const int half = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
+  int mb, tile;
+  mx_tile(a, (a.M + 32 * MI - 1) / (32 * MI), (a.N + kBigCols - 1) / kBigCols, &mb, &tile);
+  const int n0 = tile * kBigCols, m0 = mb * 32 * MI;
+  const int64_t K = (int64_t)a.nb * kMxBlock, piece = (int64_t)a.M * K;
+  const int groups = a.nb >> 2, n = a.pieces * groups;
+  // rows behind the ends read the last row: their outputs are not stored
+  const uint8_t* xs[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r = 4 * (wave * MI + i) + g, m = min(m0 + r, a.M - 1);
+    const int h = ((r & 3) << 2) | ((r >> 2) & 3);
+    xs[i] = reinterpret_cast<const uint8_t*>(a.x + (a.pieces - 1) * piece + m * K) + ((l15 ^ h) << 4);
+  }
+  const int wr = lane >> 2;
+  const uint8_t* ws = a.codes + ((int64_t)min(n0 + 16 * wave + wr, a.N - 1) * a.nb + ((lane & 3) ^ ((0x78 >> (2 * (wr >> 2))) & 3))) * 16;
+  const uint8_t* ss = a.scales + (int64_t)min(n0 + 64 * wn + lane, a.N - 1) * a.nb;  // (waves 0 and 1)
+  const unsigned base = mfl::lds_addr(lds);
+  int at = 0, slot = 0;  // the next stage's group of its piece, and its place
+  auto issue = [&]() {
+    const unsigned st = __builtin_amdgcn_readfirstlane(base + slot * kStage);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) big_dma16(xs[i] + at * 256, st + (wave * MI + i) * 1024);
+    big_dma16(ws + at * 64, st + kX + wave * 1024);
+    if (wave < 2) big_dma4(ss + at * 4, st + kX + kW + wave * 256);
+    slot = slot + 1 == S ? 0 : slot + 1;
+    if (++at == groups) {
+      at = 0;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) xs[i] -= piece * 2;
+    }
+  };
+  f32x4 acc[MI][4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int h = ((l15 & 3) << 2) | (l15 >> 2);
+  const unsigned xr = (16 * MI * wm + l15) * 256, q0 = ((4 * g + 2 * half) ^ h) << 4, q1 = ((4 * g + 2 * half + 1) ^ h) << 4;
+  const unsigned wo = kX + (64 * wn + l15) * 64 + ((g ^ ((0x78 >> (2 * (l15 >> 2))) & 3)) << 4) + 8 * half;
+  const unsigned so = kX + kW + wn * 256 + l15 * 4;
+  for (int t = 0; t < S - 1 && t < n; ++t) issue();
+  int use = 0;
+  for (int t = 0; t < n; ++t) {
+    if (t + 1 == n) mx_wait_vm<0>();
+    else if (wave < 2) mx_wait_vm<L + 1>();
+    else mx_wait_vm<L>();
+    mfl::barrier_keep_vm();  // every wave's part of stage t is there, and stage t - 1 has been read
+    asm volatile("" ::: "memory");  // no read moves up
+    if (t + S - 1 < n) issue();
+    const unsigned sb = base + use * kStage;
+    use = use + 1 == S ? 0 : use + 1;
+    u32x4 x[MI][2];
+    u32x2 w[4];
+    unsigned sc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = lds_at<u32x2>(sb + wo + j * 1024);
+      sc[j] = lds_at<unsigned>(sb + so + j * 64);
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      x[i][0] = lds_at<u32x4>(sb + xr + q0 + i * 4096);
+      x[i][1] = lds_at<u32x4>(sb + xr + q1 + i * 4096);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float s = mx_scale((sc[j] >> (8 * g)) & 255u);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const u16x8 f = mx_fragment(w[j][q], s);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) acc[i][j] = mfl::mma16<bf16_t>(f, __builtin_bit_cast(u16x8, x[i][q]), acc[i][j]);
+      }
+    }
+  }
+  // each half keeps MI / 2 of the row fragments and takes the other half's sums for them
+  __syncthreads();
+  constexpr int H = MI / 2;
+  f32x4* part = reinterpret_cast<f32x4*>(lds) + lane;
+#pragma unroll
+  for (int i = 0; i < H; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 lo = acc[i][j], hi = acc[i + H][j];
+      part[((wave * H + i) * 4 + j) * 64] = half ? lo : hi;
+    }
+  __syncthreads();
+  O* y = static_cast<O*>(a.y);
+  const bool vec = a.N % 4 == 0;
+#pragma unroll
+  for (int i = 0; i < H; ++i) {
+    const int m = m0 + 16 * (MI * wm + i + (half ? H : 0)) + l15;
+    if (m >= a.M) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 o = part[(((wave ^ 4) * H + i) * 4 + j) * 64], lo = acc[i][j], hi = acc[i + H][j];
+      float sum[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = o[e] + (half ? hi : lo)[e];
+      const int c = n0 + 64 * wn + 16 * j + 4 * g;
+      O* to = y + (int64_t)m * a.N + c;
+      if (vec && c < a.N) {
+        if (a.bias) {
+          const float4 b = *reinterpret_cast<const float4*>(a.bias + c);
+          sum[0] += b.x, sum[1] += b.y, sum[2] += b.z, sum[3] += b.w;
+        }
+        st4(to, sum);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < a.N) st1<O>(to + e, sum[e] + (a.bias ? a.bias[c + e] : 0.f));
+      }
+    }
   }
 }
 
@@ -834,9 +995,12 @@ hipError_t mx_launch(K kernel, int rows, int tiles, int waves, size_t lds, const
   return hipGetLastError();
 }
 
+// rows of a workgroup's tile
+int mx_rows(int mt) { return mt > kMxBig ? 32 * (mt - kMxBig) : 16 * (mt % kMxLds); }
+
 // row blocks (of M rows) whose activations, rows of `bytes`, take at most 2 MB
 int mx_group(int M, int mt, int64_t bytes) {
-  const int rows = 16 * (mt % kMxLds);
+  const int rows = mx_rows(mt);
   return rows == 0 ? 1 : (int)std::min<int64_t>(ceil_div(M, rows), std::max<int64_t>(1, (2 << 20) / (rows * bytes)));
 }
 
@@ -847,17 +1011,18 @@ bool mx_lds_ok(const uint8_t* scales, int nb) { return nb % 4 == 0 && reinterpre
 // Planning.  A variant is a tile, + kMxLds in its rows where the operands go through LDS (rows of whole groups of four
 // blocks); 0 is decoding the weight and the tiled GEMM.  Every variant is priced by its workgroups' rounds over 256 CUs
 // and a round's time, fitted to MI355X measurements (us, bf16 activations):
-//   forward      rows   1     16    32    64    128   333   700   1500       decoded: 128   700   1500  4064
-//   4096 x 4096         4.8   4.9   5.9   7.5   10.5  26    51    100                 31    58    79    134
-//   11008 x 4096        6.9   8.3   9.8   18    27    66    124   256                 49    137   217   376
-//   768 x 2048          3.7   3.7   3.8   3.8   4.3   5.8   11    18                  17    22    26    35
+//   forward      rows   1     16    32    64    128   333   700   1500  4064    decoded: 128   700   1500  4064
+//   4096 x 4096         4.8   4.9   5.9   7.5   10.5  23    35    59    139              31    58    79    130
+//   11008 x 4096        6.9   8.3   9.8   18    23    55    71    154   365              49    137   217   365
+//   768 x 2048          3.7   3.7   3.8   3.8   4.3   5.7   11    14    21               17    22    26    35
+//   (up to 32-row tiles from 333 rows on: 4096 x 4096 26, 51, 100; 11008 x 4096 66, 124, 256)
 //   gradient (N -> K)
 //   4096 -> 4096        14    14    14    15    17    34    50    99                  29    60    85    139
 //   11008 -> 4096       33    34    34    35    38    74    113   231                 49    116   215   346
 // (direct, without LDS: forward 4096 x 4096 5.0, 13 at 24 rows, 41 at 100; gradient 19 .. 21 up to 100 rows).
 
 // the tiled GEMM's 256 x 256 ping-pong tile (one workgroup a CU) or its 128 x 128 tile (two a CU) by the rounds that their
-// workgroups need: a 32-deep step of a round takes 1.0 / 0.62 us, a split another pass over fp32 partial sums
+// workgroups need: a 32-deep step of a round takes 0.92 / 0.62 us, a split another pass over fp32 partial sums
 double mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
   double best = 1e30;
   *tile = 3;
@@ -869,7 +1034,7 @@ double mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
     for (int s : {1, 2, 4, 8}) {
       if (s > 1 && K / s < 512) break;
       const int slots = t == 8 ? 256 : 512;
-      double us = (double)((tiles * s + slots - 1) / slots) * ceil_div(ceil_div(K, 32), s) * (t == 8 ? 1.0 : 0.62);
+      double us = (double)((tiles * s + slots - 1) / slots) * ceil_div(ceil_div(K, 32), s) * (t == 8 ? 0.92 : 0.62);
       if (s > 1) us += 4.0 + (double)M * N * 4.0 * (s + 1) / 4e6;
       if (us < best) {
         best = us;
@@ -891,7 +1056,7 @@ double decoded_us(int M, int n, int k, int64_t weight) {
 
 }  // namespace
 
-void mx_nt_plan(int M, int N, int nb, bool lds, int* mt, int* nt) {
+void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
   // a round's time is a + b * groups; two or more workgroups a CU (whole = false) fill its rounds evenly
   static const struct {
     int mt, nt;
@@ -899,12 +1064,13 @@ void mx_nt_plan(int M, int N, int nb, bool lds, int* mt, int* nt) {
     bool whole;
   } kTiles[] = {{2, 4, 1.07, 0.217, true}, {2, 2, 0.6, 0.14, true}, {1, 4, 0.2, 0.1625, true}, {1, 2, 0.23, 0.096, false},
                 {1, 1, 0.2, 0.07, false}};
-  const int K = 32 * nb;
+  const int K = 32 * nb, rows = pieces * M;
+  const double join = pieces > 1 ? 2.5 + (double)M * N * (4 * pieces + 4) / 3.5e6 : 0.0;  // not in 128-column tiles
   double best = 1e30;
   for (const auto& t : kTiles) {
     if (!lds) break;
-    const double w = (double)ceil_div(M, 16 * t.mt) * ceil_div(N, 16 * t.nt) / 256.0;
-    const double us = 2.5 + (t.a + t.b * (nb / 4)) * std::max(1.0, t.whole ? std::ceil(w) : w);
+    const double w = (double)ceil_div(rows, 16 * t.mt) * ceil_div(N, 16 * t.nt) / 256.0;
+    const double us = join + 2.5 + (t.a + t.b * (nb / 4)) * std::max(1.0, t.whole ? std::ceil(w) : w);
     if (us < best) {
       best = us;
       *mt = t.mt + kMxLds;
@@ -912,12 +1078,25 @@ void mx_nt_plan(int M, int N, int nb, bool lds, int* mt, int* nt) {
     }
   }
   if (!lds) {  // direct: 250 TFLOP/s in 2 x 4 tiles where they fill the chip
-    const bool wide = M > 16 && (int64_t)ceil_div(M, 32) * ceil_div(N, 64) >= 160;
+    const bool wide = rows > 16 && (int64_t)ceil_div(rows, 32) * ceil_div(N, 64) >= 160;
     *mt = wide ? 2 : 1;
     *nt = wide ? 4 : 1;
-    best = 2.5 + 2.0 * M * N * K / 250e6;
+    best = join + 2.5 + 2.0 * rows * N * K / 250e6;
   }
-  if (decoded_us(M, N, K, (int64_t)N * K) < best) *mt = *nt = 0;
+  for (int mi : {2, 4}) {
+    if (!lds) break;
+    // a stage takes 1.06 us in a CU's one 128-row workgroup, 0.63 in one 64-row workgroup and 1.17 in the two that fit
+    const double w = (double)ceil_div(M, 32 * mi) * ceil_div(N, 128) / 256.0, last = w - 2 * std::floor(w / 2);
+    const double round = mi == 4 ? 1.06 * std::ceil(w)
+                                 : 1.17 * std::floor(w / 2) + (last > 0 ? 0.63 + 0.54 * std::max(0.0, last - 1) : 0.0);
+    const double us = 4.0 + round * (nb / 4) * pieces;
+    if (us < best) {
+      best = us;
+      *mt = kMxBig + mi;
+      *nt = kBigCols / 16;
+    }
+  }
+  if (join + decoded_us(rows, N, K, (int64_t)N * K) < best) *mt = *nt = 0;
 }
 
 void mx_nn_plan(int M, int N, int nb, bool lds, int* mt) {
@@ -930,13 +1109,19 @@ void mx_nn_plan(int M, int N, int nb, bool lds, int* mt) {
 }
 
 hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
-                 int out_dtype, void* y, hipStream_t stream, int mt, int nt) {
+                 int out_dtype, void* y, hipStream_t stream, int mt, int nt, int pieces) {
   if (M == 0 || N == 0) return hipSuccess;
-  if (out_dtype != kBF16 && out_dtype != kF32) return hipErrorInvalidValue;
-  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, bias, y, M, N, nb, 0, 0, mx_group(M, mt, (int64_t)64 * nb)};
-  if (mt % kMxLds == 0 || nt <= 0) return hipErrorInvalidValue;
-  const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = ceil_div(N, 16 * nt);
-  if (mt > kMxLds && !mx_lds_ok(scales, nb)) return hipErrorInvalidValue;
+  if (mx_rows(mt) == 0 || nt <= 0 || (mt > kMxLds && !mx_lds_ok(scales, nb))) return hipErrorInvalidValue;
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, bias, y, M, N, nb, 0, 0, mx_group(M, mt, (int64_t)64 * nb), pieces};
+  const int rows = ceil_div(M, mx_rows(mt)), tiles = ceil_div(N, 16 * nt);
+#define HYP_MX_NT_BIG(MI)                                                                                      \
+  if (mt == kMxBig + MI && nt == kBigCols / 16)                                                                \
+    return out_dtype == kBF16  ? mx_launch(mx_nt_big_k<MI, bf16_t>, rows, tiles, 8, mx_nt_big_bytes<MI>(), a, stream) \
+           : out_dtype == kF16 ? mx_launch(mx_nt_big_k<MI, f16_t>, rows, tiles, 8, mx_nt_big_bytes<MI>(), a, stream) \
+                               : mx_launch(mx_nt_big_k<MI, float>, rows, tiles, 8, mx_nt_big_bytes<MI>(), a, stream);
+  HYP_MX_NT_BIG(2) HYP_MX_NT_BIG(4)
+#undef HYP_MX_NT_BIG
+  if (pieces != 1 || (out_dtype != kBF16 && out_dtype != kF32)) return hipErrorInvalidValue;
 #define HYP_MX_NT(MT, NT)                                                                                      \
   if (mt == MT && nt == NT) {                                                                                  \
     const size_t lds = sizeof(float) * kMxWaves * MT * NT * 256;                                               \
@@ -960,7 +1145,7 @@ hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t*
                  int out_dtype, void* y, hipStream_t stream, int mt) {
   if (M == 0 || cols == 0) return hipSuccess;
   if ((out_dtype != kBF16 && out_dtype != kF32) || ld % 8 != 0) return hipErrorInvalidValue;
-  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld, mx_group(M, mt, 2 * ld)};
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld, mx_group(M, mt, 2 * ld), 1};
   if (mt % kMxLds == 0) return hipErrorInvalidValue;
   const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = ceil_div(cols, 128);
   if (mt > kMxLds && (!mx_lds_ok(scales, nb) || ld % 128 != 0)) return hipErrorInvalidValue;

@@ -92,12 +92,12 @@ def test_every_tile_gives_the_same_product(M, N, K):
     w = quantize_mxfp4(torch.randn(N, K, generator=g).to(DEV))
     W = decoded(w.codes, w.scales, K).to(DEV)
     b = torch.randn(N, generator=g).to(DEV)
-    for dtype in (torch.bfloat16, torch.float32):
+    for dtype in DTYPES:
         x, dy = torch.randn(M, K, generator=g).to(dtype).to(DEV), torch.randn(M, N, generator=g).to(dtype).to(DEV)
         xd, dd = x.double(), dy.double()
         want = xd @ W.t() + b.double()
         bound = product_bound(xd, W.t(), dtype) + (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * (b.double().abs() + want.abs())
-        lds = [] if w.scales.shape[1] % 4 else [(9, 1), (9, 2), (9, 4), (10, 2), (10, 4)]
+        lds = [] if w.scales.shape[1] % 4 else [(9, 1), (9, 2), (9, 4), (10, 2), (10, 4), (18, 8), (20, 8)]
         for mt, nt in [(0, 0), (1, 1), (2, 4)] + lds:
             y = C.mx_linear(x, w.codes, w.scales, b, 16 * mt + nt)
             assert ((y.double() - want).abs() <= bound).all(), (mt, nt)
