@@ -166,15 +166,21 @@ at::Tensor mx_linear_dgrad(const at::Tensor& dy, const at::Tensor& codes, const 
   const int64_t M = dy.size(0), N = codes.size(0), nb = scales.size(1), P = pieces_of(dy.scalar_type());
   const auto dt = P == 1 ? at::kBFloat16 : at::kFloat;
   int mt;
-  hyp::mx_nn_plan((int)(P * M), (int)N, (int)nb, lds_ok(scales), &mt);
+  hyp::mx_nn_plan((int)M, (int)N, (int)nb, (int)P, lds_ok(scales), &mt);
   if (tile >= 0) mt = (int)tile;
   const int64_t unit = mt > hyp::kMxLds ? 128 : 8;  // the product through LDS takes whole groups of the reduction
   const at::Tensor dp = pieces(dy, (N + unit - 1) / unit * unit);
   at::Tensor dx;
+  if (mt > hyp::kMxBig) {
+    dx = at::empty({M, K}, dy.options());
+    HYP_CHECK_HIP(hyp::mx_nn(dp.data_ptr(), dp.size(1), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), (int)M, (int)N,
+                             (int)nb, (int)K, dtype_code(dx), dx.data_ptr(), cur_stream(), mt, (int)P));
+    return dx;
+  }
   if (mt > 0) {
     dx = at::empty({P * M, K}, dp.options().dtype(dt));
     HYP_CHECK_HIP(hyp::mx_nn(dp.data_ptr(), dp.size(1), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), (int)(P * M),
-                             (int)N, (int)nb, (int)K, dtype_code(dt), dx.data_ptr(), cur_stream(), mt));
+                             (int)N, (int)nb, (int)K, dtype_code(dt), dx.data_ptr(), cur_stream(), mt, 1));
   } else {
     dx = tiled(dp, N, decoded(codes, scales), true, 32 * nb, nullptr, dt);
     if (P == 1) return 32 * nb == K ? dx : dx.narrow(1, 0, K).contiguous();

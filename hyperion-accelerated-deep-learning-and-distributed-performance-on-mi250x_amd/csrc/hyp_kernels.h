@@ -175,13 +175,14 @@ constexpr int kMxLds = 8, kMxBig = 16;
 hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
                  int out_dtype, void* y, hipStream_t stream, int mt, int nt, int pieces);
 // y [M, cols] (bf16 / fp32) = x [M, N] (bf16; rows of stride ld, zeros from N to it) times the 4-bit weight [N, 32 nb], in
-// tiles of 16 mt x 128: mt 1 (ld % 8 == 0), or through LDS (mt + kMxLds; also ld % 128 == 0) 1 or 2
+// tiles of 16 mt x 128: mt 1 (ld % 8 == 0), or through LDS (mt + kMxLds; also ld % 128 == 0) 1 or 2; or
+// kMxBig + MI as above
 hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, int cols,
-                 int out_dtype, void* y, hipStream_t stream, int mt);
+                 int out_dtype, void* y, hipStream_t stream, int mt, int pieces);
 // the tile of mx_nt / mx_nn for a product, 0 where decoding the weight and the tiled GEMM are faster (lds: the weight
 // allows the products through LDS); the tiled GEMM's (tile, splits) for it and their time in us
 void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt);
-void mx_nn_plan(int M, int N, int nb, bool lds, int* mt);
+void mx_nn_plan(int M, int N, int nb, int pieces, bool lds, int* mt);
 double mx_gemm_plan(int M, int N, int K, int* tile, int* splits);
 }  // namespace hyp
 

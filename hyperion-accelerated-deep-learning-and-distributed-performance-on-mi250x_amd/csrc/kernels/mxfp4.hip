@@ -521,7 +521,7 @@ __device__ __forceinline__ V lds_at(unsigned addr) {
 }
 
 template <int MI>
-constexpr int mx_nt_big_bytes() {
+constexpr int mx_big_bytes() {
   return kBigStages * (MI * 8192 + 8192 + 512);
 }
 
@@ -920,6 +920,138 @@ __global__ __launch_bounds__(kLdsWaves * 64) void mx_nn_lds_k(const MxArgs a) {
   }
 }
 
+// ---- the data gradient in tiles of 32 MI rows -------------------------------------------------------------
+// As the forward's 128-column tiles: 8 waves share the ring, waves 4 i + q own the i-th half of the rows and the q-th 32
+// weight rows of a stage, all 128 columns; the decoding and the transposition of a fragment are paid once for MI of them.
+// The four partial sums meet in LDS: wave q keeps the rows 4 g + q of every 16, 8 consecutive columns a lane.
+template <int MI, typename O>
+__global__ __launch_bounds__(512) void mx_nn_big_k(const MxArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int kX = MI * 8192, kW = 8192, kStage = kX + kW + 512, S = kBigStages;
+  constexpr int L = MI + 1;  // DMA instructions of a wave and stage; waves 0 and 1 also bring the scales
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+  const int wm = wave >> 2, q = wave & 3;
+  int mb, tile;
+  mx_tile(a, (a.M + 32 * MI - 1) / (32 * MI), (a.cols + kBigCols - 1) / kBigCols, &mb, &tile);
+  const int k0 = tile * kBigCols, m0 = mb * 32 * MI;
+  const int64_t piece = (int64_t)a.M * a.ld;
+  const int groups = (a.N + 127) >> 7, n = a.pieces * groups;
+  // rows behind the ends repeat the last one: outputs that are not stored, weight rows that meet zeros of x
+  const uint8_t* xs[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r = 4 * (wave * MI + i) + g, m = min(m0 + r, a.M - 1);
+    xs[i] = reinterpret_cast<const uint8_t*>(a.x + (a.pieces - 1) * piece + m * a.ld) + ((l15 ^ (r & 15)) << 4);
+  }
+  const int wrow = 32 * (wave >> 1) + 8 * ((lane >> 2) & 3) + 4 * (wave & 1) + (lane >> 4), srow = 64 * wave + lane;
+  const uint8_t* ws = a.codes + (int64_t)tile * 64 + (lane & 3) * 16;
+  const uint8_t* ss = a.scales + tile * 4;
+  const unsigned base = mfl::lds_addr(lds);
+  int at = 0, slot = 0;  // the next stage's group of its piece, and its place
+  auto issue = [&]() {
+    const unsigned st = __builtin_amdgcn_readfirstlane(base + slot * kStage);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) big_dma16(xs[i] + at * 256, st + (wave * MI + i) * 1024);
+    big_dma16(ws + (int64_t)min(at * 128 + wrow, a.N - 1) * a.nb * 16, st + kX + wave * 1024);
+    if (wave < 2) big_dma4(ss + (int64_t)min(at * 128 + srow, a.N - 1) * a.nb, st + kX + kW + wave * 256);
+    slot = slot + 1 == S ? 0 : slot + 1;
+    if (++at == groups) {
+      at = 0;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) xs[i] -= piece * 2;
+    }
+  };
+  f32x4 acc[MI][8];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const unsigned turn = 8 * (l15 >> 2) + 9;  // rotates the scale byte of this lane's block to a float's exponent
+  const unsigned xo = (16 * MI * wm + l15) * 256 + (((4 * q + g) ^ l15) << 4);
+  const unsigned wo = kX + q * 2048 + g * 64 + l15 * 4, so = kX + kW + q * 128 + g * 32;
+  for (int t = 0; t < S - 1 && t < n; ++t) issue();
+  int use = 0;
+  for (int t = 0; t < n; ++t) {
+    if (t + 1 == n) mx_wait_vm<0>();
+    else if (wave < 2) mx_wait_vm<L + 1>();
+    else mx_wait_vm<L>();
+    mfl::barrier_keep_vm();  // every wave's part of stage t is there, and stage t - 1 has been read
+    asm volatile("" ::: "memory");  // no read moves up
+    if (t + S - 1 < n) issue();
+    const unsigned sb = base + use * kStage;
+    use = use + 1 == S ? 0 : use + 1;
+    u32x4 x[MI], s[2];
+    union {
+      u16x8 v;
+      unsigned w[4];
+    } row[8], f;  // row[r].w[p]: columns 2 p, 2 p + 1 of weight row r
+    unsigned w[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) w[r] = lds_at<unsigned>(sb + wo + r * 256);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) s[r] = lds_at<u32x4>(sb + so + r * 16);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) x[i] = lds_at<u32x4>(sb + xo + i * 4096);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const unsigned b = s[r >> 2][r & 3];
+      row[r].v = mx_fragment(w[r], __uint_as_float(__builtin_amdgcn_alignbit(b, b, turn) & 0x7f800000u));
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p)  // rows 2 p, 2 p + 1 of column c
+        f.w[p] = __builtin_amdgcn_perm(row[2 * p + 1].w[c >> 1], row[2 * p].w[c >> 1], (c & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) acc[i][c] = mfl::mma16<bf16_t>(__builtin_bit_cast(u16x8, x[i]), f.v, acc[i][c]);
+    }
+  }
+  constexpr int H = MI / 2;  // 16-row fragments a round of the exchange
+  f32x4* part = reinterpret_cast<f32x4*>(lds) + lane;
+  O* y = static_cast<O*>(a.y);
+  const int k = k0 + 8 * l15;
+#pragma unroll
+  for (int round = 0; round < 2; ++round) {
+    __syncthreads();  // the ring, or the last round's sums, have been read
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {  // wave q's sums for wave p, in the place that leaves q's own out
+      if (p == q) continue;
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const auto& v = acc[round * H + i];
+        f32x4* to = part + ((wave * 3 + p - (p > q)) * H + i) * 128;
+        to[0] = f32x4{v[0][p], v[1][p], v[2][p], v[3][p]};
+        to[64] = f32x4{v[4][p], v[5][p], v[6][p], v[7][p]};
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const auto& v = acc[round * H + i];
+      float sum[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) sum[c] = q == 0 ? v[c][0] : q == 1 ? v[c][1] : q == 2 ? v[c][2] : v[c][3];
+      for (int p = 0; p < 4; ++p) {
+        if (p == q) continue;
+        const f32x4* from = part + (((4 * wm + p) * 3 + q - (q > p)) * H + i) * 128;
+        const f32x4 lo = from[0], hi = from[64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += lo[e], sum[4 + e] += hi[e];
+      }
+      const int m = m0 + 16 * (MI * wm + round * H + i) + 4 * g + q;
+      if (m >= a.M) continue;
+      O* to = y + (int64_t)m * a.cols + k;
+      if (a.cols % 8 == 0) {
+        if (k < a.cols) Vec8<O>::store(to, sum);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (k + c < a.cols) st1<O>(to + c, sum[c]);
+      }
+    }
+  }
+}
+
 }  // namespace
 
 hipError_t mx_quantize(int dtype, const void* x, int64_t ld, int64_t rows, int cols, uint8_t* codes, uint8_t* scales,
@@ -1015,10 +1147,12 @@ bool mx_lds_ok(const uint8_t* scales, int nb) { return nb % 4 == 0 && reinterpre
 //   4096 x 4096         4.8   4.9   5.9   7.5   10.5  23    35    59    139              31    58    79    130
 //   11008 x 4096        6.9   8.3   9.8   18    23    55    71    154   365              49    137   217   365
 //   768 x 2048          3.7   3.7   3.8   3.8   4.3   5.7   11    14    21               17    22    26    35
-//   (up to 32-row tiles from 333 rows on: 4096 x 4096 26, 51, 100; 11008 x 4096 66, 124, 256)
+//   (at most 32-row tiles from 333 rows on: forward 4096 x 4096 26, 51, 100, 11008 x 4096 66, 124, 256; gradient
+//   4096 -> 4096 34, 50, 99, 11008 -> 4096 74, 111, 225)
 //   gradient (N -> K)
-//   4096 -> 4096        14    14    14    15    17    34    50    99                  29    60    85    139
-//   11008 -> 4096       33    34    34    35    38    74    113   231                 49    116   215   346
+//   4096 -> 4096        14    14    14    15    17    28    37    69    149             29    60    85    138
+//   11008 -> 4096       33    34    34    35    38    66    86    169   389             49    116   215   340
+//   4096 -> 11008             16          19    27    62    84    180   412             50    140   242   384
 // (direct, without LDS: forward 4096 x 4096 5.0, 13 at 24 rows, 41 at 100; gradient 19 .. 21 up to 100 rows).
 
 // the tiled GEMM's 256 x 256 ping-pong tile (one workgroup a CU) or its 128 x 128 tile (two a CU) by the rounds that their
@@ -1054,6 +1188,20 @@ double decoded_us(int M, int n, int k, int64_t weight) {
   return 5.0 + (double)weight * 0.375e-6 + mx_gemm_plan(M, n, k, &tile, &splits);
 }
 
+// 128-column tiles of 128 or 64 rows (*mi 4 or 2): a stage takes `one128` us in the one 128-row workgroup that fits a CU,
+// `one64` in a 64-row one alone and `two64` in two
+double big_us(int M, int cols, int stages, double one128, double one64, double two64, int* mi) {
+  const double w4 = (double)ceil_div(M, 128) * ceil_div(cols, 128) / 256.0, w2 = (double)ceil_div(M, 64) * ceil_div(cols, 128) / 256.0;
+  const double last = w2 - 2 * std::floor(w2 / 2);
+  const double r4 = one128 * (w4 <= 1 ? 0.93 : std::ceil(w4));  // (a lone round runs a little faster)
+  const double r2 = two64 * std::floor(w2 / 2) + (last > 1 ? one64 + 0.8 * (two64 - one64) : last > 0 ? one64 : 0.0);
+  *mi = r2 < r4 ? 2 : 4;
+  return 4.0 + std::min(r2, r4) * stages;
+}
+
+// joining the pieces' products, which the 128-column tiles need not do
+double join_us(int M, int cols, int pieces) { return pieces > 1 ? 2.5 + (double)M * cols * (4 * pieces + 4) / 3.5e6 : 0.0; }
+
 }  // namespace
 
 void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
@@ -1065,7 +1213,7 @@ void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
   } kTiles[] = {{2, 4, 1.07, 0.217, true}, {2, 2, 0.6, 0.14, true}, {1, 4, 0.2, 0.1625, true}, {1, 2, 0.23, 0.096, false},
                 {1, 1, 0.2, 0.07, false}};
   const int K = 32 * nb, rows = pieces * M;
-  const double join = pieces > 1 ? 2.5 + (double)M * N * (4 * pieces + 4) / 3.5e6 : 0.0;  // not in 128-column tiles
+  const double join = join_us(M, N, pieces);
   double best = 1e30;
   for (const auto& t : kTiles) {
     if (!lds) break;
@@ -1083,29 +1231,31 @@ void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
     *nt = wide ? 4 : 1;
     best = join + 2.5 + 2.0 * rows * N * K / 250e6;
   }
-  for (int mi : {2, 4}) {
-    if (!lds) break;
-    // a stage takes 1.06 us in a CU's one 128-row workgroup, 0.63 in one 64-row workgroup and 1.17 in the two that fit
-    const double w = (double)ceil_div(M, 32 * mi) * ceil_div(N, 128) / 256.0, last = w - 2 * std::floor(w / 2);
-    const double round = mi == 4 ? 1.06 * std::ceil(w)
-                                 : 1.17 * std::floor(w / 2) + (last > 0 ? 0.63 + 0.54 * std::max(0.0, last - 1) : 0.0);
-    const double us = 4.0 + round * (nb / 4) * pieces;
-    if (us < best) {
-      best = us;
-      *mt = kMxBig + mi;
-      *nt = kBigCols / 16;
-    }
+  int mi;
+  if (lds && big_us(M, N, nb / 4 * pieces, 1.06, 0.63, 1.17, &mi) < best) {
+    best = big_us(M, N, nb / 4 * pieces, 1.06, 0.63, 1.17, &mi);
+    *mt = kMxBig + mi;
+    *nt = kBigCols / 16;
   }
   if (join + decoded_us(rows, N, K, (int64_t)N * K) < best) *mt = *nt = 0;
 }
 
-void mx_nn_plan(int M, int N, int nb, bool lds, int* mt) {
-  const int K = 32 * nb;
-  lds = lds && N >= 1024 && N % 128 == 0;  // else the direct product is as fast, and activations need no padding
-  const int rows = lds && (int64_t)ceil_div(M, 16) * ceil_div(nb, 4) > 256 ? 2 : 1;
-  const int64_t rounds = (ceil_div(M, 16 * rows) * (int64_t)ceil_div(nb, 4) + 255) / 256;
-  const double us = 2.5 + rounds * (lds ? 1.0 + (rows == 2 ? 0.48 : 0.36) * N / 128 : 0.5 + 0.6 * N / 128);
-  *mt = decoded_us(M, K, N, (int64_t)N * K) < us ? 0 : rows + (lds ? kMxLds : 0);
+void mx_nn_plan(int M, int N, int nb, int pieces, bool lds, int* mt) {
+  const int K = 32 * nb, all = pieces * M;
+  const double join = join_us(M, K, pieces);
+  const bool ring = lds && N >= 1024 && N % 128 == 0;  // else the direct product is as fast, and activations need no padding
+  const int rows = ring && (int64_t)ceil_div(all, 16) * ceil_div(nb, 4) > 256 ? 2 : 1;
+  const int64_t rounds = (ceil_div(all, 16 * rows) * (int64_t)ceil_div(nb, 4) + 255) / 256;
+  double best = join + 2.5 + rounds * (ring ? 1.0 + (rows == 2 ? 0.48 : 0.36) * N / 128 : 0.5 + 0.6 * N / 128);
+  *mt = rows + (ring ? kMxLds : 0);
+  int mi;
+  const double padding = pieces == 1 && N % 128 != 0 ? 2.5 + (double)M * N * 4 / 4.5e6 : 0.0;
+  const double big = padding + big_us(M, K, ceil_div(N, 128) * pieces, 1.13, 0.68, 1.28, &mi);
+  if (lds && big < best) {
+    best = big;
+    *mt = kMxBig + mi;
+  }
+  if (join + decoded_us(all, K, N, (int64_t)N * K) < best) *mt = 0;
 }
 
 hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
@@ -1116,9 +1266,9 @@ hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int
   const int rows = ceil_div(M, mx_rows(mt)), tiles = ceil_div(N, 16 * nt);
 #define HYP_MX_NT_BIG(MI)                                                                                      \
   if (mt == kMxBig + MI && nt == kBigCols / 16)                                                                \
-    return out_dtype == kBF16  ? mx_launch(mx_nt_big_k<MI, bf16_t>, rows, tiles, 8, mx_nt_big_bytes<MI>(), a, stream) \
-           : out_dtype == kF16 ? mx_launch(mx_nt_big_k<MI, f16_t>, rows, tiles, 8, mx_nt_big_bytes<MI>(), a, stream) \
-                               : mx_launch(mx_nt_big_k<MI, float>, rows, tiles, 8, mx_nt_big_bytes<MI>(), a, stream);
+    return out_dtype == kBF16  ? mx_launch(mx_nt_big_k<MI, bf16_t>, rows, tiles, 8, mx_big_bytes<MI>(), a, stream) \
+           : out_dtype == kF16 ? mx_launch(mx_nt_big_k<MI, f16_t>, rows, tiles, 8, mx_big_bytes<MI>(), a, stream) \
+                               : mx_launch(mx_nt_big_k<MI, float>, rows, tiles, 8, mx_big_bytes<MI>(), a, stream);
   HYP_MX_NT_BIG(2) HYP_MX_NT_BIG(4)
 #undef HYP_MX_NT_BIG
   if (pieces != 1 || (out_dtype != kBF16 && out_dtype != kF32)) return hipErrorInvalidValue;
@@ -1142,13 +1292,20 @@ hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int
 }
 
 hipError_t mx_nn(const void* x, int64_t ld, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, int cols,
-                 int out_dtype, void* y, hipStream_t stream, int mt) {
+                 int out_dtype, void* y, hipStream_t stream, int mt, int pieces) {
   if (M == 0 || cols == 0) return hipSuccess;
-  if ((out_dtype != kBF16 && out_dtype != kF32) || ld % 8 != 0) return hipErrorInvalidValue;
-  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld, mx_group(M, mt, 2 * ld), 1};
-  if (mt % kMxLds == 0) return hipErrorInvalidValue;
-  const int rows = ceil_div(M, 16 * (mt % kMxLds)), tiles = ceil_div(cols, 128);
+  if (ld % 8 != 0 || mx_rows(mt) == 0) return hipErrorInvalidValue;
+  MxArgs a{static_cast<const bf16_t*>(x), codes, scales, nullptr, y, M, N, nb, cols, ld, mx_group(M, mt, 2 * ld), pieces};
+  const int rows = ceil_div(M, mx_rows(mt)), tiles = ceil_div(cols, 128);
   if (mt > kMxLds && (!mx_lds_ok(scales, nb) || ld % 128 != 0)) return hipErrorInvalidValue;
+#define HYP_MX_NN_BIG(MI)                                                                                      \
+  if (mt == kMxBig + MI)                                                                                       \
+    return out_dtype == kBF16  ? mx_launch(mx_nn_big_k<MI, bf16_t>, rows, tiles, 8, mx_big_bytes<MI>(), a, stream) \
+           : out_dtype == kF16 ? mx_launch(mx_nn_big_k<MI, f16_t>, rows, tiles, 8, mx_big_bytes<MI>(), a, stream) \
+                               : mx_launch(mx_nn_big_k<MI, float>, rows, tiles, 8, mx_big_bytes<MI>(), a, stream);
+  HYP_MX_NN_BIG(2) HYP_MX_NN_BIG(4)
+#undef HYP_MX_NN_BIG
+  if (pieces != 1 || (out_dtype != kBF16 && out_dtype != kF32)) return hipErrorInvalidValue;
   if (mt == 1) {
     const size_t lds = sizeof(float) * kMxWaves * 2048;
     return out_dtype == kBF16 ? mx_launch(mx_nn_k<bf16_t>, rows, tiles, kMxWaves, lds, a, stream)

@@ -101,7 +101,7 @@ def test_every_tile_gives_the_same_product(M, N, K):
         for mt, nt in [(0, 0), (1, 1), (2, 4)] + lds:
             y = C.mx_linear(x, w.codes, w.scales, b, 16 * mt + nt)
             assert ((y.double() - want).abs() <= bound).all(), (mt, nt)
-        for mt in [0, 1] + ([9, 10] if lds else []):
+        for mt in [0, 1] + ([9, 10, 18, 20] if lds else []):
             dx = C.mx_linear_dgrad(dy, w.codes, w.scales, K, mt)
             assert ((dx.double() - dd @ W).abs() <= product_bound(dd, W, dtype)).all(), mt
 
