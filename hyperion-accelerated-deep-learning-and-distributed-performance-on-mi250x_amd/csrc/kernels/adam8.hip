@@ -31,6 +31,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLane = 8;  // elements a lane; 32 lanes hold a block
+// 1 / 127^2 and 1 / 255^4: products with them, not quotients (PyTorch divides by a number with a product on the GPU and a
+// quotient on the CPU, which differ in the last bit and, at those halves, in the scale)
+constexpr double kUnitM = 1.0 / 16129.0, kUnitV = 1.0 / 4228250625.0;
 
 struct Adam8Args {
   float lr, eps, wd, ln_b1, ln_b2;
@@ -143,7 +146,7 @@ __global__ __launch_bounds__(kThreads) void adam8_mt_k(const int64_t* __restrict
     load_lane<G>(g + i0, left, gv);
     mw = load_codes(mq + i0, left);
     vw = load_codes(vq + i0, left);
-    const double m_step = (double)ms[blk] / 16129.0, v_step = (double)vs[blk] / 4228250625.0;
+    const double m_step = (double)ms[blk] * kUnitM, v_step = (double)vs[blk] * kUnitV;
     double md[8], vd[8];
     unsigned m_top = 0, v_top = 0;
 #pragma unroll
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void adam8_mt_k(const int64_t* __restrict
     const float m_s = kept_scale(half_max(m_top)), v_s = kept_scale(half_max(v_top));
     const bool m_live = m_s > 0.f, v_live = v_s > 0.f;  // neither 0 nor NaN
     const float m_inv = m_live ? __builtin_amdgcn_rcpf(m_s) : 0.f, v_inv = v_live ? __builtin_amdgcn_rcpf(v_s) : 0.f;
-    const double m_unit = (double)m_s * (1.0 / 16129.0), v_unit = (double)v_s * (1.0 / 4228250625.0);
+    const double m_unit = (double)m_s * kUnitM, v_unit = (double)v_s * kUnitV;
     uint32_t mo[2] = {0u, 0u}, vo[2] = {0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void adam8_values_k(const int64_t* __rest
         vw |= (uint32_t)vq[i0 + i] << (8 * i);
       }
     }
-    const double m_step = (double)ms[i0 >> 8] / 16129.0, v_step = (double)vs[i0 >> 8] / 4228250625.0;
+    const double m_step = (double)ms[i0 >> 8] * kUnitM, v_step = (double)vs[i0 >> 8] * kUnitV;
     float m[4], v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

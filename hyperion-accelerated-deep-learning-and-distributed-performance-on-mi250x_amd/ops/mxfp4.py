@@ -13,8 +13,9 @@ is one of 0, .5, 1, 1.5, 2, 3, 4, 6 with a sign (e2m1), two to a byte, the first
   activations are split into two or three bf16 numbers whose sum they are, and lose nothing either.
   The weight is frozen: it has no gradient.
 
-Products up to a few hundred rows run on one launch that decodes the codes on their way to the matrix
-instructions; larger ones decode the weight to bf16 once (a buffer of the call) and run on the tiled GEMM.
+The products decode the codes on their way to the matrix instructions, in one launch (fp16 and fp32 activations are
+split by another); the largest, where it is faster, decode the weight to bf16 once (a buffer of the call) and run on the
+tiled GEMM.
 """
 from __future__ import annotations
 

@@ -91,7 +91,8 @@ def _encode8(x: torch.Tensor, levels: int, second: bool) -> Tuple[torch.Tensor, 
 def _decode8(q: torch.Tensor, s: torch.Tensor, levels: int, second: bool) -> torch.Tensor:
     b = _in_blocks(q.double())
     b = b * b * (b * b if second else torch.sign(b))
-    return (b * (s.double() / float(levels) ** (4 if second else 2))[:, None]).view(-1)[:q.numel()]
+    unit = 1.0 / float(levels) ** (4 if second else 2)  # (a product: quotients by a number differ between CPU and GPU)
+    return (b * (s.double() * unit)[:, None]).view(-1)[:q.numel()]
 
 
 def _row_major(x: torch.Tensor, moved) -> torch.Tensor:

@@ -204,3 +204,29 @@ def test_learning_rates_as_tensors():
             opt.step()
         results.append(p.detach().clone())
     assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+
+
+def test_scales_at_exact_halves():
+    """0.9 S + 0.1 g is halfway between two fp32 numbers for many g a few steps from S: CPU and GPU round alike, also in the
+    PyTorch path on the GPU."""
+    n = 2048
+    S = 1 + torch.arange(n) / n
+    g = torch.zeros(n, 256)
+    g[:, 7] = S * (1 + 2.0 ** -23 * (torch.arange(n) % 31))
+    state = {"exp_avg_q": torch.zeros(n, 256, dtype=torch.int8), "exp_avg_sq_q": torch.zeros(n, 256, dtype=torch.uint8),
+             "exp_avg_scale": S.clone(), "exp_avg_sq_scale": S.square()}
+    state["exp_avg_q"][:, 7], state["exp_avg_sq_q"][:, 7] = 127, 255
+    results = []
+    for dev, backend in (("cpu", "hyperion"), (DEV, "hyperion"), (DEV, "torch")):
+        p = torch.nn.Parameter(torch.zeros(n, 256, device=dev))
+        opt = FusedAdamW([p], lr=1e-3, state_bits=8)
+        opt.load_state_dict({"state": {0: {k: v.reshape(-1).to(dev) for k, v in state.items()}}, "hyperion_step": 5,
+                             "param_groups": opt.state_dict()["param_groups"]})
+        p.grad = g.to(dev)
+        with pytest.MonkeyPatch.context() as mp:
+            mp.setenv("HYPERION_KERNELS", backend)
+            opt.step()
+        results.append({k: opt.state[p][k].cpu() for k in state})
+    for other in results[1:]:
+        for k in state:
+            assert torch.equal(results[0][k], other[k]), k
