@@ -1232,8 +1232,8 @@ void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
     best = join + 2.5 + 2.0 * rows * N * K / 250e6;
   }
   int mi;
-  if (lds && big_us(M, N, nb / 4 * pieces, 1.06, 0.63, 1.17, &mi) < best) {
-    best = big_us(M, N, nb / 4 * pieces, 1.06, 0.63, 1.17, &mi);
+  if (lds && big_us(M, N, nb / 4 * pieces, 1.03, 0.63, 1.17, &mi) < best) {
+    best = big_us(M, N, nb / 4 * pieces, 1.03, 0.63, 1.17, &mi);
     *mt = kMxBig + mi;
     *nt = kBigCols / 16;
   }
