@@ -384,10 +384,10 @@ __device__ __forceinline__ void mx_read_w(unsigned wa, unsigned sa, u32x4 (&w)[2
 __device__ __forceinline__ void mx_read_w(unsigned wa, unsigned sa, u32x4 (&w)[4], unsigned (&s)[4]) {
   asm volatile(
       "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b128 %2, %8 offset:2048\n\t"
-      "ds_read_b128 %3, %8 offset:3072\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:64\n\t"
+      "ds_read_b128 %3, %8 offset:%10\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:64\n\t"
       "ds_read_b32 %6, %9 offset:128\n\tds_read_b32 %7, %9 offset:192\n\ts_waitcnt lgkmcnt(0)"
       : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
-      : "v"(wa), "v"(sa)
+      : "v"(wa), "v"(sa), "i"(3 * 1024)
       : "memory");
 }
 

@@ -189,3 +189,33 @@ def test_empty_sizes(M, N, K):
     dx, db = torch.autograd.grad(y.sum(), [x, b])
     assert dx.shape == x.shape and (N or not dx.any())
     assert torch.equal(db, torch.full_like(b, M))
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(700, 4096, 4096, torch.bfloat16), (333, 2049, 1024, torch.bfloat16),
+                                         (600, 2048, 1152, torch.float32), (1500, 1000, 2048, torch.float16),
+                                         (4096, 4096, 1024, torch.bfloat16)])
+def test_many_rows(M, N, K, dtype):
+    """The planned products of longer batches against the oracle, eager and replayed."""
+    g = torch.Generator().manual_seed(M + N)
+    w = quantize_mxfp4(torch.randn(N, K, generator=g).to(DEV))
+    W = decoded(w.codes, w.scales, K).to(DEV)
+    x, dy = torch.randn(M, K, generator=g).to(DEV, dtype), torch.randn(M, N, generator=g).to(DEV, dtype)
+
+    def step(t):
+        t = t.detach().requires_grad_(True)
+        y = mxfp4_linear(t, w)
+        return [y.detach(), torch.autograd.grad(y, t, dy)[0]]
+
+    y, dx = step(x)
+    assert ((y.double() - x.double() @ W.t()).abs() <= product_bound(x.double(), W.t(), dtype)).all()
+    assert ((dx.double() - dy.double() @ W).abs() <= product_bound(dy.double(), W, dtype)).all()
+    static = x.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for i in range(3):
+        static.copy_(torch.roll(x, i, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step(static)))
