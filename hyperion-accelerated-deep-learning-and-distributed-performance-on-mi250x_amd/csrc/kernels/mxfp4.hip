@@ -492,7 +492,7 @@ __global__ __launch_bounds__(kLdsWaves * 64) void mx_nt_lds_k(const MxArgs a) {
 // For more rows: 8 waves share a ring of stages (one barrier a stage) over 32 MI rows and 128 columns, so that a
 // decoded fragment meets MI fragments of activations.  Waves 4 h + 2 i + j own the i-th half of the rows and the j-th of
 // the columns for half h of every block's elements: two waves a SIMD (one alone issues at half rate), whose
-// sums meet in LDS.  4064 x 11008 x 4096 in 368 us (1.0 PFLOP/s, the tiled GEMM's rate without a decoded weight),
+// sums meet in LDS.  2048 x 11008 x 4096 in 194 us (0.95 PFLOP/s; decoded weight and tiled GEMM 237),
 // 512 x 4096 x 4096 in 25 us against 36 in 32-row tiles.  Halves a barrier apart (one multiplies while the other
 // reads) were slower, 37.6 against 34.6 us at 512 rows, and so was every wave bringing its own scales (42 against 36 us at
 // 700 rows in 64-row tiles).  The images are those above.  x holds P pieces [M, 32 nb] whose sum the activations are: the
@@ -1232,8 +1232,8 @@ void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
     best = join + 2.5 + 2.0 * rows * N * K / 250e6;
   }
   int mi;
-  if (lds && big_us(M, N, nb / 4 * pieces, 1.03, 0.63, 1.17, &mi) < best) {
-    best = big_us(M, N, nb / 4 * pieces, 1.03, 0.63, 1.17, &mi);
+  if (lds && big_us(M, N, nb / 4 * pieces, 1.1, 0.63, 1.17, &mi) < best) {
+    best = big_us(M, N, nb / 4 * pieces, 1.1, 0.63, 1.17, &mi);
     *mt = kMxBig + mi;
     *nt = kBigCols / 16;
   }
