@@ -116,11 +116,12 @@ __device__ __forceinline__ float largest(const float (&v)[N]) {
   return mx;
 }
 
-// order of the alternatives: larger logit first (NaN above everything, -0 = +0), then the lower id
+// order of the alternatives: larger logit first (NaN above everything, -0 = +0), then the lower id.  Every key is below
+// ~0, the sweeps' start, and above 0: the row's k <= V keys are distinct, so each of k sweeps finds one.
 __device__ __forceinline__ uint64_t top_key(float z, int id) {
   const uint32_t b = __float_as_uint(z + 0.f);
   uint32_t k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  if (z != z) k = 0xffffffffu;
+  if (z != z) k = 0xfffffffeu;
   return ((uint64_t)k << 32) | (0xffffffffu - (uint32_t)id);
 }
 __device__ __forceinline__ uint64_t shfl_max64(uint64_t v) {

@@ -195,3 +195,15 @@ def test_other_stream_and_graph_replays():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, step(static)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,k", [(1, 1), (3, 3), (32, 32), (32, 5), (700, 32), (9001, 8)])
+def test_nan_at_the_first_token(V, k, dtype):
+    # alone, with others behind it, everywhere, with an infinity; as many alternatives as tokens among the sizes
+    z, t, a, b = rows(5, V, dtype, V)
+    z[0, 0] = math.nan
+    z[1] = math.nan
+    z[2, [0, V // 2, V - 1]] = math.nan
+    z[3, 0], z[3, V - 1] = math.nan, math.inf
+    compare(z.to(DEV), t, a, b, k)

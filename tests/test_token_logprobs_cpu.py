@@ -52,6 +52,15 @@ def test_masked_empty_and_poisoned_rows():
     compare(z, t, a, b, 4)
 
 
+@pytest.mark.parametrize("V,k", [(1, 1), (3, 3), (32, 5)])
+def test_nan_at_the_first_token(V, k):
+    z, t, a, b = rows(4, V, torch.float32, V)
+    z[0, 0] = math.nan
+    z[1] = math.nan
+    z[2, [0, V - 1]] = math.nan
+    compare(z, t, a, b, k)
+
+
 def test_gradient_against_differences():
     z, t, a, b = rows(3, 11, torch.float32)
 
