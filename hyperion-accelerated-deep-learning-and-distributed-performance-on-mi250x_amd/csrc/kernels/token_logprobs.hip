@@ -206,8 +206,8 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
   const int head = min(a.V, (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T));
   const int nv = (a.V - head) / N, tail = head + nv * N;  // 16-byte pieces; elements [0, head) and [tail, V) are single
   const u32x4* body = reinterpret_cast<const u32x4*>(z + head);
-  const int one = tid < head ? tid : tid - head + tail;   // this thread's single element, if any
-  const bool has_one = one < a.V && tid < head + a.V - tail;
+  const bool has_one = tid < a.V - tail + head;           // (differences first: V may be close to 2^31)
+  const int one = tid < head ? tid : has_one ? tail + (tid - head) : 0;  // this thread's single element, if any
   const float lone = has_one ? ld1<T>(z + one) : -INFINITY;
   Run run{-INFINITY, 0.f, 0.f};
   float best = -INFINITY;
@@ -372,6 +372,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_lp_bwd_k(const LpArgs a, co
   const bool ignored = tgt == a.ignore;
   T* g = dz + row * a.V;
   const int nv = a.V / N, tail = nv * N;
+  const bool lone = (int)threadIdx.x < a.V - tail;  // one of the last elements is this thread's (V may be close to 2^31)
   const int v0 = chunk * (kBwdThreads * kBwdU) + threadIdx.x;
   const float m = a.stats[3 * row], ls = a.stats[3 * row + 1], h = a.stats[3 * row + 2];
   float wl = 0.f, wh = 0.f;  // both 0 in an ignored or empty row
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_lp_bwd_k(const LpArgs a, co
       const int v = v0 + i * kBwdThreads;
       if (v < nv) *reinterpret_cast<u32x4a*>(g + (int64_t)v * N) = zero;
     }
-    if (chunk == 0 && tail + (int)threadIdx.x < a.V) st1<T>(g + tail + threadIdx.x, 0.f);
+    if (chunk == 0 && lone) st1<T>(g + tail + threadIdx.x, 0.f);
     return;
   }
   const T* z = row_ptr<T>(a, row);
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_lp_bwd_k(const LpArgs a, co
       *reinterpret_cast<u32x4a*>(g + (int64_t)v * N) = close16(x, (const T*)nullptr);
     }
   }
-  if (chunk == 0 && tail + (int)threadIdx.x < a.V)
+  if (chunk == 0 && lone)
     st1<T>(g + tail + threadIdx.x, grad(ld1<T>(z + tail + threadIdx.x), tail + threadIdx.x));
 }
 
@@ -478,7 +479,7 @@ hipError_t token_logprobs_bwd(int dtype, const void* z, int64_t s0, int64_t s1, 
   a.stats = const_cast<float*>(stats);
   HYP_DISPATCH_FLOAT(dtype, T, {
     const int per = kBwdThreads * kBwdU * Row16<T>::N;
-    const int64_t chunks = (V + per - 1) / per;
+    const int64_t chunks = ((int64_t)V + per - 1) / per;
     if (rows * chunks >= kTokenRowsMax) return hipErrorInvalidValue;
     hipLaunchKernelGGL((token_lp_bwd_k<T>), dim3(rows * chunks), dim3(kBwdThreads), 0, stream, a, dlogp, dent,
                        static_cast<T*>(dz), (int)chunks);

@@ -207,3 +207,23 @@ def test_nan_at_the_first_token(V, k, dtype):
     z[2, [0, V // 2, V - 1]] = math.nan
     z[3, 0], z[3, V - 1] = math.nan, math.inf
     compare(z.to(DEV), t, a, b, k)
+
+
+def test_longest_row():
+    # 2^31 - 2 logits, the most that a row may have: equal but for the last two, one of which is the target
+    V = (1 << 31) - 2
+    z = torch.zeros(1, V, dtype=torch.bfloat16, device=DEV)
+    z[0, V - 2:] = torch.tensor([15.0, 20.0])
+    z.requires_grad_(True)
+    o = token_logprobs(z, torch.tensor([V - 1], device=DEV))
+    total = V - 2 + math.exp(15.0) + math.exp(20.0)
+    want = 20.0 - math.log(total)
+    # sums of whole powers of two up to 2^31 are exact, the others and the logarithm are rounded a few times
+    assert abs(float(o.logprobs.detach()) - want) <= 16 * 2.0 ** -24 * math.log(total)
+    g, = torch.autograd.grad(o.logprobs.sum(), z)
+    p = torch.tensor([1.0, math.exp(15.0), math.exp(20.0)], dtype=torch.float64) / total
+    got = torch.stack([g[0, :1].double().cpu()[0], *g[0, V - 2:].double().cpu()])
+    expect = torch.stack([-p[0], -p[1], 1 - p[2]])
+    # rounded to bf16 (2^-8); exponents of up to 31 are rounded a few times in fp32
+    assert ((got - expect).abs() <= expect.abs() * (2.0 ** -8 + 256 * 2.0 ** -24) + 2.0 ** -22 * p[2]).all()
+    assert bool((g[0, :V - 2] == g[0, 0]).all())
