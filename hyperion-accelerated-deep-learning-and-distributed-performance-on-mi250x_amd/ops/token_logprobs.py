@@ -39,11 +39,11 @@ class TokenLogprobs(NamedTuple):
 def _reference_fwd(z, target, k, ignore_index, inv_t):
     """PyTorch oracle of the forward kernel over [rows, V]: (logprobs, entropy, stats, top logprobs, top ids)."""
     V = z.shape[1]
-    y = z.float() * inv_t
     keep = target != ignore_index
-    m = y.amax(1)
+    m = z.amax(1).float()
     empty = m == -math.inf  # (a NaN makes m NaN)
-    d = y - torch.where(empty, torch.zeros_like(m), m)[:, None]
+    # the difference first, as in the kernel: divided by the temperature, the type's lowest value would be -inf
+    d = (z.float() - torch.where(empty, torch.zeros_like(m), m)[:, None]) * inv_t
     e = torch.exp(d)
     s = e.sum(1)
     logs = torch.where(empty, torch.full_like(s, math.inf), torch.log(s))
@@ -69,7 +69,7 @@ def _reference_bwd(z, target, stats, ignore_index, inv_t, dlogp, dent):
     wl = torch.where(live, zero if dlogp is None else dlogp[:, None], zero)
     wl = torch.where(live & ~inside, torch.full_like(wl, math.nan), wl)
     wh = torch.where(live, zero if dent is None else dent[:, None], zero)
-    q = z.float() * inv_t - m - logs
+    q = (z.float() - m) * inv_t - logs
     p = torch.exp(q)
     dz = torch.where(p == 0, torch.zeros_like(p), -p * (wl + wh * (q + h)))
     dz = dz.scatter_add(1, torch.where(inside[:, 0], target, torch.zeros_like(target))[:, None], wl)

@@ -52,6 +52,25 @@ def test_masked_empty_and_poisoned_rows():
     compare(z, t, a, b, 4)
 
 
+@pytest.mark.parametrize("temperature", [0.5, 0.7, 1.3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_logits_at_the_ends_of_their_type(dtype, temperature):
+    z, t, a, b = rows(7, 65, dtype)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z[0] = low
+    z[1] = low
+    z[1, 3:] = -math.inf
+    t[1] = 2
+    z[2, 5:] = low
+    t[2] = 1
+    z[3] = high
+    z[4, 7] = 0.8 * high  # one token is certain
+    t[4] = 7
+    z[5, 1::2] = low / 2
+    t[5] = 4
+    compare(z, t, a, b, 1, temperature)
+
+
 @pytest.mark.parametrize("V,k", [(1, 1), (3, 3), (32, 5)])
 def test_nan_at_the_first_token(V, k):
     z, t, a, b = rows(4, V, torch.float32, V)
