@@ -13,7 +13,9 @@ lower id) with their log probabilities.  Sums are fp32 whatever the logits' type
 * A row whose target is ``ignore_index`` gives 0 everywhere, ids -1 and a zero gradient.
 * -inf logits (a masked vocabulary) have probability 0 and no gradient.  A row with nothing else has
   log probabilities -inf, entropy 0 and a zero gradient.
-* A NaN or +inf logit makes its row's results NaN, and so does a target outside the vocabulary.
+* A NaN or +inf logit makes its row's results and its whole gradient NaN.  A target outside the vocabulary
+  makes its row's log probability and whole gradient NaN (masked logits among them, as does a NaN that comes
+  back as the gradient of either result); the entropy and the alternatives do not depend on it.
 """
 from __future__ import annotations
 
@@ -27,6 +29,7 @@ from . import _native
 
 TOP_MAX = 32  # hyp::kTokenTopMax
 TOP_VOCAB = 1 << 18  # hyp::kTokenTopVocab
+FLOOR = -200 * math.log(2.0)  # hyp::kFloor as a natural logarithm: exp of it is 0 in fp32
 
 
 class TokenLogprobs(NamedTuple):
@@ -71,7 +74,7 @@ def _reference_bwd(z, target, stats, ignore_index, inv_t, dlogp, dent):
     wh = torch.where(live, zero if dent is None else dent[:, None], zero)
     q = (z.float() - m) * inv_t - logs
     p = torch.exp(q)
-    dz = torch.where(p == 0, torch.zeros_like(p), -p * (wl + wh * (q + h)))
+    dz = -p * (wl + wh * (q.clamp(min=FLOOR) + h))  # (finite in a masked place: 0 unless the row's gradient is NaN)
     dz = dz.scatter_add(1, torch.where(inside[:, 0], target, torch.zeros_like(target))[:, None], wl)
     dz = torch.where((target != ignore_index)[:, None], dz * inv_t, torch.zeros_like(dz))
     return dz.to(z.dtype)

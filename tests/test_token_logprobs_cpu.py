@@ -71,6 +71,18 @@ def test_logits_at_the_ends_of_their_type(dtype, temperature):
     compare(z, t, a, b, 1, temperature)
 
 
+def test_a_poisoned_row_has_no_gradient_but_nan():
+    z, t, a, b = rows(3, 40, torch.float32)
+    z[:, 20:] = -math.inf
+    t[0], t[1], t[2] = 40, 3, 5
+    b[1] = math.nan
+    zd = z.requires_grad_(True)
+    o = token_logprobs(zd, t, top_k=3)
+    g, = torch.autograd.grad([o.logprobs, o.entropy], [zd], [a, b])
+    assert torch.isnan(o.logprobs[0]) and torch.isfinite(o.entropy).all() and torch.isfinite(o.top_logprobs).all()
+    assert torch.isnan(g[:2]).all() and torch.isfinite(g[2]).all() and (g[2, 20:] == 0).all()
+
+
 @pytest.mark.parametrize("V,k", [(1, 1), (3, 3), (32, 5)])
 def test_nan_at_the_first_token(V, k):
     z, t, a, b = rows(4, V, torch.float32, V)
