@@ -24,6 +24,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _MOD = None
 _ERR: Optional[BaseException] = None
@@ -195,9 +196,17 @@ def apply_fn(fn, *args, needs_grad: bool = True):
     argument needs a gradient (``needs_grad=False``) — ``fn.forward`` on a stand-in
     ctx: the same kernels without the autograd-node bookkeeping, which costs ~10 us of host time per
     op and made the launch-bound fused inference of LM-768 slower than torch eager."""
-    if needs_grad and torch.is_grad_enabled():
+    if (needs_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0 and _kernel_tangents(args)):
         return fn.apply(*args)
     return fn.forward(_InferCtx(), *args)
+
+
+def _kernel_tangents(args) -> bool:
+    """Whether a tensor that a kernel may read carries a forward-mode tangent, which its output would lack:
+    autograd then refuses the call, as the ops have no forward-mode derivative.  (The PyTorch path on the CPU
+    carries tangents by itself.)"""
+    return backend() != "torch" and any(
+        isinstance(t, torch.Tensor) and t.is_cuda and forward_ad.unpack_dual(t).tangent is not None for t in args)
 
 
 _COUNTS: dict = {}

@@ -70,3 +70,26 @@ def test_trainer_graphed_and_eager_agree(tmp_path):
         losses.append(r["history"][0]["loss"])
     # the dropout streams differ between the two; the losses are those of six small steps from one start
     assert abs(losses[0] - losses[1]) < 0.05 * losses[0]
+
+
+def test_forward_mode_is_refused_not_lost():
+    from torch.autograd import forward_ad as fw
+
+    from hyperion.ops.layernorm import layer_norm
+    from hyperion.ops.mxfp4 import mxfp4_linear, quantize_mxfp4
+    from hyperion.ops.token_logprobs import token_logprobs
+
+    w = quantize_mxfp4(torch.randn(16, 64, device="cuda"))
+    x, b = torch.randn(3, 64, device="cuda"), torch.randn(16, device="cuda")
+    scale = torch.ones(64, device="cuda")
+    t = torch.zeros(3, dtype=torch.long, device="cuda")
+    calls = [lambda d: mxfp4_linear(d, w, b), lambda d: mxfp4_linear(x, w, d[0, :16]), lambda d: token_logprobs(d, t)]
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        for call in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call(d)
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            layer_norm(d.bfloat16(), scale.bfloat16(), scale.bfloat16(), 1e-5)
+        assert torch.equal(mxfp4_linear(x, w, b), mxfp4_linear(d.detach().clone(), w, b))

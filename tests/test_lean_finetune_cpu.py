@@ -76,3 +76,21 @@ def test_trainer_with_a_4_bit_base(tmp_path):
     assert r["history"][0]["steps"] == 2 and r["mode"].endswith("mxfp4")
     with pytest.raises(ValueError, match="base_format"):
         train_llama_fsdp(0, 1, base_dir=str(tmp_path), lora=False, base_format="mxfp4")
+
+
+def test_forward_mode_on_the_cpu_paths():
+    from torch.autograd import forward_ad as fw
+
+    from hyperion.ops.mxfp4 import mxfp4_linear, quantize_mxfp4
+    from hyperion.ops.token_logprobs import token_logprobs
+
+    torch.manual_seed(4)
+    w, x, dx = quantize_mxfp4(torch.randn(16, 64)), torch.randn(3, 64), torch.randn(3, 64)
+    t = torch.tensor([1, 2, 63])
+    with fw.dual_level():
+        d = fw.make_dual(x, dx)
+        y = fw.unpack_dual(mxfp4_linear(d, w)).tangent
+        torch.testing.assert_close(y, dx @ w.dequantize(torch.float32).t(), atol=1e-5, rtol=1e-5)
+        lp = fw.unpack_dual(token_logprobs(d, t).logprobs).tangent
+    want = (dx.gather(1, t[:, None])[:, 0] - (torch.softmax(x, 1) * dx).sum(1))
+    torch.testing.assert_close(lp, want, atol=1e-5, rtol=1e-5)
