@@ -6,13 +6,14 @@
 // block keep relative precision:
 //   m:  int8 q in [-127, 127],  m = q |q| S / 127^2,   q = sign(m) round(127 (|m| / S)^(1/2))
 //   v: uint8 q in [0, 255],     v = q^4 S / 255^4,     q = round(255 (v / S)^(1/4)), at least 1 where v > 0
-// (levels 127^2 and 255^4 apart in a block; v > 0 never becomes 0, which would divide by eps alone).
+// where a half goes to the lower code (levels 127^2 and 255^4 apart in a block; v > 0 never becomes 0, which would
+// divide by eps alone).
 // A scale below the smallest normal number is kept as 0 and its block as zeros; a scale that is not
 // finite is kept as NaN: its block is NaN.
 //
 // The new moments m' = b1 m + (1 - b1) g and v' = b2 v + (1 - b2) g^2 are fp64, and so is the decision
-// between two codes: the fp32 square roots only find k = floor(r), and |m'| is then compared with the
-// border S ((k + 1/2) / 127)^2 (v' with S ((k + 1/2) / 255)^4).  The codes are thus those of the exact
+// between two codes: the fp32 square roots only find k = floor(r), and |m'| becomes k + 1 where it is above the
+// border S ((k + 1/2) / 127)^2 (v' above S ((k + 1/2) / 255)^4).  The codes are thus those of the exact
 // formula, whatever the instructions' rounding.  The fp64 operations are those of the PyTorch path, one by
 // one and uncontracted, so that scales and codes are the same bits on CPU and GPU (0.9 S + 0.1 g is
 // often exactly halfway between two fp32 numbers, where a fused product would round the other way).

@@ -72,15 +72,24 @@ def _in_blocks(x: torch.Tensor) -> torch.Tensor:
     return torch.nn.functional.pad(x, (0, -x.numel() % STATE_BLOCK)).view(-1, STATE_BLOCK)
 
 
+def _unit(levels: int, second: bool) -> float:
+    """What a block's largest magnitude is multiplied with: a product, as quotients by a number differ between CPU and GPU."""
+    return 1.0 / float(levels) ** (4 if second else 2)
+
+
 def _encode8(x: torch.Tensor, levels: int, second: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """fp64 [n] -> (codes [n], fp32 scales)"""
+    """fp64 [n] -> (codes [n], fp32 scales).  As in the kernel, the root only finds k = floor(r) and x is then compared
+    with the border of k and k + 1, which itself belongs to k."""
     b = _in_blocks(x)
     s = b.abs().amax(1).float() if b.numel() else b.new_zeros(0).float()
     s = torch.where(s < torch.finfo(torch.float32).tiny, torch.zeros_like(s), s)
     s = torch.where(torch.isfinite(s), s, torch.full_like(s, math.nan))
     live = (s > 0)[:, None]
+    unit = torch.where(live, s.double()[:, None] * _unit(levels, second), torch.zeros_like(b))
     r = torch.where(live, b.abs() / s.double()[:, None], torch.zeros_like(b)).sqrt()
-    q = torch.round((r.sqrt() if second else r) * levels).clamp(max=levels)
+    k = torch.floor((r.sqrt() if second else r) * levels).clamp(max=levels)
+    h = (k + 0.5) * (k + 0.5) if second else k * k + k + 0.25
+    q = torch.where(live, k + (b.abs() > unit * (h * h if second else h)), torch.zeros_like(b))
     if second:
         q = torch.where(live & (b > 0) & (q < 1), torch.ones_like(q), q)
     else:
@@ -91,8 +100,7 @@ def _encode8(x: torch.Tensor, levels: int, second: bool) -> Tuple[torch.Tensor, 
 def _decode8(q: torch.Tensor, s: torch.Tensor, levels: int, second: bool) -> torch.Tensor:
     b = _in_blocks(q.double())
     b = b * b * (b * b if second else torch.sign(b))
-    unit = 1.0 / float(levels) ** (4 if second else 2)  # (a product: quotients by a number differ between CPU and GPU)
-    return (b * (s.double() * unit)[:, None]).view(-1)[:q.numel()]
+    return (b * (s.double() * _unit(levels, second))[:, None]).view(-1)[:q.numel()]
 
 
 def _row_major(x: torch.Tensor, moved) -> torch.Tensor:

@@ -190,3 +190,32 @@ def test_memory_format_changes():
     o2.load_state_dict(opt.state_dict())
     for k in ("exp_avg", "exp_avg_sq", "master"):
         assert o2.state[q][k].stride() == q.stride() and torch.equal(o2.state[q][k], opt.state[p][k])
+
+
+def at_the_borders(dev):
+    """One step with betas of 1/2 from nothing, whose moments lie exactly on the borders between two codes."""
+    k = torch.arange(127.0)
+    g = torch.zeros(4, 256)
+    g[0, :127], g[0, 127] = (k + 0.5) ** 2, 127.0 ** 2  # m' = g / 2: the border of k and k + 1 under S = 127^2 / 2
+    g[1] = -g[0]
+    g[2, 0], g[2, 1:6] = 1.0, torch.tensor([0.25, -0.25, 0.25 + 2.0 ** -25, 0.25 - 2.0 ** -25, 0.0])  # v' / S = 1 / 16
+    g[3, :3] = torch.tensor([1.0, 0.25, 0.0])  # m' / S = 1 / 4: 63.5
+    p = torch.nn.Parameter(torch.zeros(4, 256, device=dev))
+    opt = FusedAdam([p], betas=(0.5, 0.5), state_bits=8)
+    p.grad = g.to(dev)
+    opt.step()
+    st = opt.state[p]
+    return st["exp_avg_q"].view(4, 256).cpu(), st["exp_avg_sq_q"].view(4, 256).cpu(), st
+
+
+def check_borders(dev):
+    m, v, _ = at_the_borders(dev)
+    k = torch.arange(127)
+    assert torch.equal(m[0, :127].long(), k) and m[0, 127] == 127  # a half goes to the lower code
+    assert torch.equal(m[1, :127].long(), -k) and m[1, 127] == -127
+    assert m[3, 1] == 63
+    assert v[2, :6].tolist() == [255, 127, 127, 128, 127, 0]
+
+
+def test_borders_between_two_codes():
+    check_borders("cpu")

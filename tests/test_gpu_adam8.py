@@ -4,7 +4,7 @@ import torch
 
 from hyperion.ops import FusedAdam, FusedAdamW, _native, clip_grad_norm_
 
-from test_adam8_cpu import run_against_oracle
+from test_adam8_cpu import at_the_borders, check_borders, run_against_oracle
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -230,3 +230,10 @@ def test_scales_at_exact_halves():
     for other in results[1:]:
         for k in state:
             assert torch.equal(results[0][k], other[k]), k
+
+
+def test_borders_between_two_codes():
+    check_borders(DEV)
+    a, b = at_the_borders("cpu")[2], at_the_borders(DEV)[2]
+    for k in ("exp_avg_q", "exp_avg_sq_q", "exp_avg_scale", "exp_avg_sq_scale"):
+        assert torch.equal(a[k], b[k].cpu()), k
