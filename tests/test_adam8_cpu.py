@@ -219,3 +219,40 @@ def check_borders(dev):
 
 def test_borders_between_two_codes():
     check_borders("cpu")
+
+
+def run_main_grads(dtype, dev, adamw):
+    """fp32 gradients (``main_grad``) of low-precision parameters with masters, step by step against the oracle."""
+    rng = np.random.default_rng(11)
+    lr, b1, b2, eps, wd = 1e-2, 0.9, 0.999, 1e-8, 0.1
+    ps = [torch.nn.Parameter(torch.tensor(rng.normal(size=s), dtype=torch.float32).to(dtype).to(dev))
+          for s in ((3, 5), (257,), (2, 8193))]
+    opt = FusedAdam(ps, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd, adamw=adamw, state_bits=8)
+    ws = [p.detach().double().reshape(-1).cpu().numpy() for p in ps]
+    ms, vs = [np.zeros(p.numel()) for p in ps], [np.zeros(p.numel()) for p in ps]
+    for t in range(1, 4):
+        for p in ps:
+            g = rng.normal(size=p.shape) * 10.0 ** rng.uniform(-6, 0, size=p.shape)
+            p.main_grad = torch.tensor(g, dtype=torch.float32).to(dev)  # (most have more digits than dtype holds)
+        opt.step()
+        for i, p in enumerate(ps):
+            g = p.main_grad.reshape(-1).cpu().numpy()
+            w1, m1, v1 = o.step(ws[i].astype(np.float32), g, ms[i], vs[i], t, lr, b1, b2, eps, wd, adamw)
+            st = opt.state[p]
+            for x, key, second, into in ((m1, "exp_avg", False, ms), (v1, "exp_avg_sq", True, vs)):
+                q, s = o.encode(x, second)
+                got, scale = st[key + "_q"].cpu().numpy().astype(np.float64), st[key + "_scale"].cpu().numpy()
+                np.testing.assert_array_equal(got, q)
+                np.testing.assert_allclose(scale, s, rtol=2.0 ** -23, atol=0)  # (one step of fp32, as above)
+                into[i] = o.decode(got, scale, second)
+            # the master: a few fp32 roundings of it, and of its update
+            got = st["master"].reshape(-1).double().cpu().numpy()
+            np.testing.assert_array_less(np.abs(got - w1), 2.0 ** -22 * np.abs(w1) + 2.0 ** -20 * np.abs(w1 - ws[i]) + 1e-30)
+            assert st["master"].dtype == torch.float32 and torch.equal(p.detach(), st["master"].to(dtype))
+            ws[i] = got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("adamw", [True, False])
+def test_fp32_gradients_of_low_precision_parameters(dtype, adamw):
+    run_main_grads(dtype, "cpu", adamw)

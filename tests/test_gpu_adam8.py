@@ -4,7 +4,7 @@ import torch
 
 from hyperion.ops import FusedAdam, FusedAdamW, _native, clip_grad_norm_
 
-from test_adam8_cpu import at_the_borders, check_borders, run_against_oracle
+from test_adam8_cpu import at_the_borders, check_borders, run_against_oracle, run_main_grads
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -237,3 +237,52 @@ def test_borders_between_two_codes():
     a, b = at_the_borders("cpu")[2], at_the_borders(DEV)[2]
     for k in ("exp_avg_q", "exp_avg_sq_q", "exp_avg_scale", "exp_avg_sq_scale"):
         assert torch.equal(a[k], b[k].cpu()), k
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("adamw", [True, False])
+def test_fp32_gradients_of_low_precision_parameters(dtype, adamw):
+    _native.reset_counters()
+    run_main_grads(dtype, DEV, adamw)
+    assert _native.counters()["adam8"] == 3
+
+
+def test_captured_moment_vectors():
+    torch.manual_seed(5)
+    ws = [torch.randn(300, 70, device=DEV).bfloat16(), torch.randn(9001, device=DEV).bfloat16()]
+    grads = [[torch.randn_like(w) for w in ws] for _ in range(6)]
+    pairs = []
+    for _ in range(2):
+        ps = [torch.nn.Parameter(w.clone()) for w in ws]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        pairs.append((ps, FusedAdamW(ps, lr=1e-2, state_bits=8)))
+
+    def load(ps, i):
+        for p, g in zip(ps, grads[i]):
+            p.grad.copy_(g)
+
+    (pa, oa), (pb, ob) = pairs
+    for ps, opt in pairs:
+        load(ps, 0)
+        opt.step(), opt.moment_vectors()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ob.step()
+        captured = ob.moment_vectors()
+    held = []
+    for i in range(1, 6):
+        load(pa, i), load(pb, i)
+        oa.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = oa.moment_vectors()
+        assert all(torch.equal(x, y) for x, y in zip(captured, want))
+        # an eager call on other state gets a table of its own and leaves the graph's as it is
+        other = {k: v.clone() for k, v in ob.state[pb[0]].items() if isinstance(v, torch.Tensor)}
+        own = dict(ob.state[pb[0]])
+        ob.state[pb[0]].update(other)
+        held.append(other)
+        assert all(torch.equal(x, y) for x, y in zip(ob.moment_vectors(), want))
+        ob.state[pb[0]].update(own)
