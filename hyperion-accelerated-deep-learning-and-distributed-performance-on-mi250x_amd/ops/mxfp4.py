@@ -152,23 +152,24 @@ class _MXLinearFn(torch.autograd.Function):
         else:
             y = x.float() @ w._rows(torch.float32, K).t()
             y = (y if bias is None else y + bias.float()).to(x.dtype)
-        ctx.w, ctx.native, ctx.xshape, ctx.bdtype = w, native, x.shape, None if bias is None else bias.dtype
+        ctx.save_for_backward(w.codes, w.scales)  # (a weight loaded before the backward is noticed there)
+        ctx.wshape, ctx.native, ctx.xshape, ctx.bdtype = w.shape, native, x.shape, None if bias is None else bias.dtype
         return y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        w = ctx.w
-        N, K = w.shape
+        codes, scales = ctx.saved_tensors
+        N, K = ctx.wshape
         dx = db = None
         if ctx.needs_input_grad[0]:
             if dy.numel() == 0 or K == 0:
                 dx = dy.new_zeros(ctx.xshape)
             elif ctx.native:
                 _native.count("mxfp4_dgrad")
-                dx = _native.native().mx_linear_dgrad(_unit_rows(dy, N), w.codes, w.scales, K).view(ctx.xshape)
+                dx = _native.native().mx_linear_dgrad(_unit_rows(dy, N), codes, scales, K).view(ctx.xshape)
             else:
-                dx = (dy.float() @ w._rows(torch.float32, K)).to(dy.dtype)
+                dx = (dy.float() @ _decode_reference(codes, scales)[:, :K]).to(dy.dtype)
         if ctx.bdtype is not None and ctx.needs_input_grad[1]:
             db = bias_grad(dy.reshape(math.prod(dy.shape[:-1]), N).contiguous(), ctx.bdtype)
         return dx, db, None

@@ -3,9 +3,10 @@ import math
 
 import pytest
 import torch
+import torch.nn as nn
 
 from hyperion.ops import _native
-from hyperion.ops.mxfp4 import MXFP4Tensor, mxfp4_linear, quantize_mxfp4
+from hyperion.ops.mxfp4 import MXFP4Linear, MXFP4Tensor, mxfp4_linear, quantize_mxfp4
 
 from mxfp4_oracle import decoded, product_bound, quantized_values
 
@@ -219,3 +220,15 @@ def test_many_rows(M, N, K, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step(static)))
+
+
+def test_a_weight_loaded_before_the_backward_is_noticed():
+    m = MXFP4Linear.from_linear(nn.Linear(64, 8).to(DEV))
+    other = MXFP4Linear.from_linear(nn.Linear(64, 8).to(DEV))
+    x = torch.randn(3, 64, device=DEV, requires_grad=True)
+    y, z = m(x), other(x)
+    m.load_state_dict(other.state_dict())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    z.sum().backward()
+    assert x.grad is not None

@@ -112,3 +112,15 @@ def test_refusals():
                 lambda: MXFP4Tensor(q.codes[:3], q.scales, q.shape), lambda: mxfp4_linear(x, q, torch.zeros(4, dtype=torch.long))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_a_weight_loaded_before_the_backward_is_noticed():
+    m = MXFP4Linear.from_linear(nn.Linear(64, 8))
+    other = MXFP4Linear.from_linear(nn.Linear(64, 8))
+    x = torch.randn(3, 64, requires_grad=True)
+    y, z = m(x), other(x)
+    m.load_state_dict(other.state_dict())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    z.sum().backward()
+    assert x.grad is not None
