@@ -100,15 +100,27 @@ def apply_lora(model: nn.Module, r: int = 16, alpha: float = 32.0, dropout: floa
 
 def quantize_base(model: nn.Module) -> nn.Module:
     """Hold every frozen plain linear layer (``nn.Linear`` or ``ops.linear.Linear``; a LoRA layer's base among
-    them) in 4 bits, in place.  Subclasses that do more (LM heads, fused activations) and layers with
-    trainable weights stay as they are."""
+    them) in 4 bits, in place.  Subclasses that do more (LM heads, fused activations), layers with
+    trainable weights and layers whose weight something else computes stay as they are.  A layer that the
+    model holds in several places stays one layer, and its forward and backward hooks stay on it."""
+    made: Dict[int, nn.Module] = {}
     adapters = {id(m) for lora in model.modules() if isinstance(lora, LoRALinear)
                 for d in (lora.lora_A, lora.lora_B) for m in d.values()}
     for mod in list(model.modules()):
-        for cname, child in list(mod.named_children()):
-            if type(child) in (nn.Linear, Linear) and not child.weight.requires_grad and id(child) not in adapters:
-                setattr(mod, cname, MXFP4Linear.from_linear(child))
+        for cname, child in list(mod._modules.items()):  # (named_children names a layer once)
+            if (type(child) in (nn.Linear, Linear) and "weight" in child._parameters and not child.weight.requires_grad
+                    and id(child) not in adapters):
+                if id(child) not in made:
+                    made[id(child)] = m = MXFP4Linear.from_linear(child)
+                    m.training = child.training
+                    for k in _HOOKS:  # the dictionaries themselves: handles that the hooks' owners hold still remove them
+                        setattr(m, k, getattr(child, k))
+                setattr(mod, cname, made[id(child)])
     return model
+
+
+_HOOKS = ("_forward_pre_hooks", "_forward_pre_hooks_with_kwargs", "_forward_hooks", "_forward_hooks_with_kwargs",
+          "_forward_hooks_always_called", "_backward_pre_hooks", "_backward_hooks", "_is_full_backward_hook")
 
 
 def lora_config_dict(r: int, alpha: float, dropout: float, targets: List[str],

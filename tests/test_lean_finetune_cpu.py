@@ -94,3 +94,37 @@ def test_forward_mode_on_the_cpu_paths():
         lp = fw.unpack_dual(token_logprobs(d, t).logprobs).tangent
     want = (dx.gather(1, t[:, None])[:, 0] - (torch.softmax(x, 1) * dx).sum(1))
     torch.testing.assert_close(lp, want, atol=1e-5, rtol=1e-5)
+
+
+def test_quantised_layers_keep_their_places_and_hooks():
+    class Two(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a = torch.nn.Linear(64, 64)
+            self.b = self.a
+            self.rest = torch.nn.ModuleList([self.a, torch.nn.Linear(64, 8)])
+            self.normed = torch.nn.utils.weight_norm(torch.nn.Linear(8, 8))
+
+        def forward(self, x):
+            return self.normed(self.rest[1](self.rest[0](self.b(self.a(x)))))
+
+    m = Two().eval()
+    for p in m.parameters():
+        p.requires_grad_(False)
+    seen = []
+    handles = [m.a.register_forward_pre_hook(lambda mod, args, kwargs: seen.append("pre"), with_kwargs=True),
+               m.a.register_forward_hook(lambda mod, args, y: y + 1.0),
+               m.a.register_full_backward_hook(lambda mod, gi, go: seen.append("grad"))]
+    normed = m.normed
+    quantize_base(m)
+    assert isinstance(m.a, MXFP4Linear) and m.b is m.a and m.rest[0] is m.a and isinstance(m.rest[1], MXFP4Linear)
+    assert m.normed is normed and not m.a.training
+    x = torch.randn(3, 64, requires_grad=True)
+    w = m.a.weight.dequantize(torch.float32)
+    torch.testing.assert_close(m.a(x), x @ w.t() + m.a.bias + 1.0, atol=1e-5, rtol=1e-5)
+    m(x).sum().backward()
+    assert seen.count("pre") == 4 and seen.count("grad") == 3
+    for h in handles:
+        h.remove()
+    torch.testing.assert_close(m.a(x), x @ w.t() + m.a.bias, atol=1e-5, rtol=1e-5)
+    assert seen.count("pre") == 4
