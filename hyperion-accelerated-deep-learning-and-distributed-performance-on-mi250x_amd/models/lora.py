@@ -111,16 +111,21 @@ def quantize_base(model: nn.Module) -> nn.Module:
             if (type(child) in (nn.Linear, Linear) and "weight" in child._parameters and not child.weight.requires_grad
                     and id(child) not in adapters):
                 if id(child) not in made:
-                    made[id(child)] = m = MXFP4Linear.from_linear(child)
-                    m.training = child.training
-                    for k in _HOOKS:  # the dictionaries themselves: handles that the hooks' owners hold still remove them
-                        setattr(m, k, getattr(child, k))
+                    made[id(child)] = _take_over(child, MXFP4Linear.from_linear(child))
                 setattr(mod, cname, made[id(child)])
     return model
 
 
 _HOOKS = ("_forward_pre_hooks", "_forward_pre_hooks_with_kwargs", "_forward_hooks", "_forward_hooks_with_kwargs",
           "_forward_hooks_always_called", "_backward_pre_hooks", "_backward_hooks", "_is_full_backward_hook")
+
+
+def _take_over(old: nn.Module, new: nn.Module) -> nn.Module:
+    """``new`` in ``old``'s mode and with its hooks."""
+    new.training = old.training
+    for k in _HOOKS:  # the dictionaries themselves: handles that the hooks' owners hold still remove them
+        setattr(new, k, getattr(old, k))
+    return new
 
 
 def lora_config_dict(r: int, alpha: float, dropout: float, targets: List[str],
@@ -184,11 +189,11 @@ def merge_lora(model: nn.Module) -> nn.Module:
                 base = child.base_layer
                 if isinstance(base, MXFP4Linear):  # the merged weight is no 4-bit one any more
                     w = child.merged_weight()
-                    full = nn.Linear(base.in_features, base.out_features, bias=False, device=w.device, dtype=w.dtype)
+                    full = Linear(base.in_features, base.out_features, bias=False, device=w.device, dtype=w.dtype)
                     full.weight.data.copy_(w)
                     full.weight.requires_grad_(False)
                     full.bias = base.bias
-                    base = full
+                    base = _take_over(base, full)
                 else:
                     base.weight.data.copy_(child.merged_weight())
                 setattr(mod, cname, base)

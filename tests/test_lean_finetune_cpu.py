@@ -128,3 +128,23 @@ def test_quantised_layers_keep_their_places_and_hooks():
         h.remove()
     torch.testing.assert_close(m.a(x), x @ w.t() + m.a.bias, atol=1e-5, rtol=1e-5)
     assert seen.count("pre") == 4
+
+
+def test_merged_layers_are_the_frameworks_own():
+    from hyperion.ops.linear import Linear
+
+    m = build("cpu", torch.float32).eval()
+    base = m.model.layers[0].self_attn.q_proj.base_layer
+    calls = []
+    handle = base.register_forward_hook(lambda mod, args, y: calls.append(mod))
+    kinds = {n: type(x) for n, x in LlamaForCausalLM(LlamaConfig.tiny()).named_modules() if n.endswith("_proj")}
+    merge_lora(m)
+    for n, x in m.named_modules():
+        if n.endswith(("q_proj", "k_proj", "v_proj", "o_proj")):
+            assert type(x) is kinds[n] is Linear and not x.training and not x.weight.requires_grad, n
+    ids, mask, _, _ = batch("cpu")
+    m(ids, mask)
+    assert calls == [m.model.layers[0].self_attn.q_proj]
+    handle.remove()
+    m(ids, mask)
+    assert len(calls) == 1
