@@ -64,8 +64,14 @@ class LoRALinear(nn.Module):
         a = self.adapter
         p = self.p if self.training else 0.0
         if isinstance(self.base_layer, MXFP4Linear):
+            # three products, each rounded to x's type once, as three layers would; scaled and added in fp32, which the
+            # fused path of a plain base does inside its one product
             t = linear(dropout(x, p, self.training), self.lora_A[a].weight)
-            return self.base_layer(x) + self.scaling[a] * linear(t, self.lora_B[a].weight)
+            y, u = self.base_layer(x), linear(t, self.lora_B[a].weight)
+            if y.is_cuda:
+                return torch.add(y, u, alpha=self.scaling[a])
+            # (on the CPU add would round the scaling to the operands' type first)
+            return torch.add(y.float(), u.float(), alpha=self.scaling[a]).to(torch.result_type(y, u))
         return lora_linear(x, self.base_layer.weight, self.base_layer.bias, self.lora_A[a].weight,
                            self.lora_B[a].weight, self.scaling[a], p)
 

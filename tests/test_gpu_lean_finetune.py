@@ -93,3 +93,10 @@ def test_forward_mode_is_refused_not_lost():
         with torch.no_grad(), pytest.raises(NotImplementedError):
             layer_norm(d.bfloat16(), scale.bfloat16(), scale.bfloat16(), 1e-5)
         assert torch.equal(mxfp4_linear(x, w, b), mxfp4_linear(d.detach().clone(), w, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_adapter_is_added_with_one_rounding(dtype):
+    from test_lean_finetune_cpu import check_one_rounding
+
+    check_one_rounding("cuda", dtype)

@@ -148,3 +148,33 @@ def test_merged_layers_are_the_frameworks_own():
     handle.remove()
     m(ids, mask)
     assert len(calls) == 1
+
+
+def check_one_rounding(dev, dtype):
+    torch.manual_seed(6)
+    layer = LoRALinear(MXFP4Linear.from_linear(torch.nn.Linear(96, 64, device=dev)), r=7, alpha=12, dropout=0.0, dtype=dtype).eval()
+    torch.nn.init.normal_(layer.lora_B["default"].weight)
+    x = torch.randn(50, 96, device=dev).to(dtype).requires_grad_(True)
+    y = layer(x)
+    with torch.no_grad():
+        base = layer.base_layer(x)
+        u = layer.lora_B["default"](layer.lora_A["default"](x)) if dev == "cpu" else None
+        if u is None:
+            from hyperion.ops.linear import linear
+
+            u = linear(linear(x, layer.lora_A["default"].weight), layer.lora_B["default"].weight)
+    want = base.double() + 12 / 7 * u.double()
+    # one rounding to dtype, and two of fp32 (the scaling and the sum) of at most |base| + 12 / 7 |u|
+    bound = torch.finfo(dtype).eps / 2 * want.abs() * (1 + 1e-6) + 2.0 ** -22 * (base.double().abs() + 2 * u.double().abs())
+    assert y.dtype == dtype and bool(((y.detach().double() - want).abs() <= bound).all())
+    dy = torch.randn(50, 64, device=dev).to(dtype)
+    gb, = torch.autograd.grad(y, layer.lora_B["default"].weight, dy)
+    want = (12 / 7 * dy.double()).t() @ layer.lora_A["default"](x).detach().double()
+    # dy scaled and rounded, the product's operand and result rounded
+    scale = (12 / 7 * dy.double()).abs().t() @ layer.lora_A["default"](x).detach().double().abs()
+    assert bool(((gb.double() - want).abs() <= 4 * torch.finfo(dtype).eps * scale).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_adapter_is_added_with_one_rounding(dtype):
+    check_one_rounding("cpu", dtype)
