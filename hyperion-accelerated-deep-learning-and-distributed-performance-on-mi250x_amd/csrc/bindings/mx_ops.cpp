@@ -188,6 +188,19 @@ at::Tensor mx_linear_dgrad(const at::Tensor& dy, const at::Tensor& codes, const 
   return P == 1 ? dx : join(dx, M, K, nullptr, dy.scalar_type());
 }
 
+// the variant that mx_linear (x [M, K], weight [N, K], rows of whole groups of four blocks) or mx_linear_dgrad plans, as
+// their `tile`, and the tiled GEMM's (tile, splits) where it is 0
+std::tuple<int64_t, int64_t, int64_t> mx_plan(int64_t M, int64_t N, int64_t K, int64_t pieces, bool dgrad) {
+  TORCH_CHECK(M >= 1 && N >= 1 && K >= 1 && M < (1 << 24) && N < (1 << 24) && K < (1 << 24) && pieces >= 1 && pieces <= 3,
+              "mx_plan: sizes in [1, 2^24), 1 to 3 pieces");
+  const int nb = (int)((K + 31) / 32);
+  int mt = 0, nt = 0, tile, splits;
+  if (dgrad) hyp::mx_nn_plan((int)M, (int)N, nb, (int)pieces, nb % 4 == 0, &mt);
+  else hyp::mx_nt_plan((int)M, (int)N, nb, (int)pieces, nb % 4 == 0, &mt, &nt);
+  hyp::mx_gemm_plan((int)(pieces * M), dgrad ? 32 * nb : (int)N, dgrad ? (int)N : 32 * nb, &tile, &splits);
+  return {dgrad ? mt : 16 * mt + nt, tile, splits};
+}
+
 }  // namespace
 
 void register_mx_ops(pybind11::module& m) {
@@ -196,6 +209,8 @@ void register_mx_ops(pybind11::module& m) {
         pybind11::arg("scales"), pybind11::arg("cols"), pybind11::arg("dtype"));
   m.def("mx_linear", &mx_linear, "x times the transposed 4-bit weight (+ bias)", pybind11::arg("x"), pybind11::arg("codes"),
         pybind11::arg("scales"), pybind11::arg("bias") = pybind11::none(), pybind11::arg("tile") = -1);
+  m.def("mx_plan", &mx_plan, "the planned variant of a product, and the tiled GEMM's tile and splits", pybind11::arg("M"),
+        pybind11::arg("N"), pybind11::arg("K"), pybind11::arg("pieces") = 1, pybind11::arg("dgrad") = false);
   m.def("mx_linear_dgrad", &mx_linear_dgrad, "dy times the 4-bit weight", pybind11::arg("dy"), pybind11::arg("codes"),
         pybind11::arg("scales"), pybind11::arg("K"), pybind11::arg("tile") = -1);
 }

@@ -492,8 +492,8 @@ __global__ __launch_bounds__(kLdsWaves * 64) void mx_nt_lds_k(const MxArgs a) {
 // For more rows: 8 waves share a ring of stages (one barrier a stage) over 32 MI rows and 128 columns, so that a
 // decoded fragment meets MI fragments of activations.  Waves 4 h + 2 i + j own the i-th half of the rows and the j-th of
 // the columns for half h of every block's elements: two waves a SIMD (one alone issues at half rate), whose
-// sums meet in LDS.  2048 x 11008 x 4096 in 194 us (0.95 PFLOP/s; decoded weight and tiled GEMM 237),
-// 512 x 4096 x 4096 in 25 us against 36 in 32-row tiles.  Halves a barrier apart (one multiplies while the other
+// sums meet in LDS.  2048 x 11008 x 4096 in 185 us in 64-row tiles, 197 in 128-row ones (1.0 PFLOP/s; decoded
+// weight and tiled GEMM 248), 450 x 4096 x 4096 in 23 us against 34 in 32-row tiles.  Halves a barrier apart (one multiplies while the other
 // reads) were slower, 37.6 against 34.6 us at 512 rows, and so was every wave bringing its own scales (42 against 36 us at
 // 700 rows in 64-row tiles).  The images are those above.  x holds P pieces [M, 32 nb] whose sum the activations are: the
 // reduction runs over the weight once for each, the smallest first, into the same fp32 sums.
@@ -1141,26 +1141,32 @@ bool mx_lds_ok(const uint8_t* scales, int nb) { return nb % 4 == 0 && reinterpre
 }  // namespace
 
 // Planning.  A variant is a tile, + kMxLds in its rows where the operands go through LDS (rows of whole groups of four
-// blocks); 0 is decoding the weight and the tiled GEMM.  Every variant is priced by its workgroups' rounds over 256 CUs
-// and a round's time, fitted to MI355X measurements (us, bf16 activations):
-//   forward      rows   1     16    32    64    128   333   700   1500  4064    decoded: 128   700   1500  4064
-//   4096 x 4096         4.8   4.9   5.9   7.5   10.5  23    35    59    139              31    58    79    130
-//   11008 x 4096        6.9   8.3   9.8   18    23    55    71    154   365              49    137   217   365
-//   768 x 2048          3.7   3.7   3.8   3.8   4.3   5.7   11    14    21               17    22    26    35
-//   (at most 32-row tiles from 333 rows on: forward 4096 x 4096 26, 51, 100, 11008 x 4096 66, 124, 256; gradient
-//   4096 -> 4096 34, 50, 99, 11008 -> 4096 74, 111, 225)
+// blocks); 0 is decoding the weight and the tiled GEMM.  Every variant is priced by its workgroups' rounds over 256 CUs:
+// a start, and for each round a part for its ends and a part for each stage of its reduction.  The prices (us) are fitted
+// to every variant's time over 28 weights (N 768 .. 11008, K 768 .. 11008) and 16 numbers of rows (1 .. 4064), bf16; within
+// 10 % for 8 shapes in 10.  Choosing by them costs 0.3 % (forward) and 0.1 % (gradient) more than the best
+// variant of each shape, on average over the 448.  Measured, us, with what was chosen:
+//   forward      rows   1     16    32    64    128   300   700   1500  4064    decoded: 128   700   1500  4064
+//   4096 x 4096       4.6   4.8   5.6   7.3   10.0  22    34    55    128          29    55    78    128
+//   11008 x 4096      6.8   7.1   9.4   17    23    35    69    150   366          50    133   231   368
+//   768 x 2048        4.0   4.0   4.0   4.0   4.2   5.2   10    13    20           17    21    25    33
+//   11008 x 2048      4.8   5.1   6.6   12    13    20    38    80    194          33    80    138   208
 //   gradient (N -> K)
-//   4096 -> 4096        14    14    14    15    17    28    37    69    149             29    60    85    138
-//   11008 -> 4096       33    34    34    35    38    66    86    169   389             49    116   215   340
-//   4096 -> 11008             16          19    27    62    84    180   412             50    140   242   384
-// (direct, without LDS: forward 4096 x 4096 5.0, 13 at 24 rows, 41 at 100; gradient 19 .. 21 up to 100 rows).
+//   4096 -> 4096      13    14    14    15    17    26    36    63    134          29    57    84    134
+//   11008 -> 4096     32    34    34    35    39    63    87    160   330          50    112   214   330
+//   4096 -> 11008     15    16    16    18    27    42    80    175   378          50    139   241   378
+//   768 -> 768        5.4   5.8   5.8   5.8   5.9   6.0   7.5   8.7   12           19    19    19    20
+// (in tiles of at most 32 rows, 1500 rows take 99 us forward at 4096 x 4096 and 96 at 4096 -> 4096; without LDS the gradient
+// takes 19 .. 21 there up to 100 rows).
 
-// the tiled GEMM's 256 x 256 ping-pong tile (one workgroup a CU) or its 128 x 128 tile (two a CU) by the rounds that their
-// workgroups need: a 32-deep step of a round takes 0.92 / 0.62 us, a split another pass over fp32 partial sums
+// the tiled GEMM's 256 x 256 ping-pong tile (one workgroup a CU) or its 128 x 128 tile (one or two a CU), chosen by the
+// rounds that their workgroups need: a 32-deep step of a round takes 0.92 / 0.62 us, a split another pass over fp32 partial
+// sums.  Returns the choice's time, with the ends of a round apart from its steps.
 double mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
   double best = 1e30;
   *tile = 3;
   *splits = 1;
+  int64_t groups = 0;
   for (int t : {8, 3}) {
     const int b = t == 8 ? 256 : 128;
     if (t == 8 && (M < 256 || N < 256)) continue;
@@ -1172,53 +1178,64 @@ double mx_gemm_plan(int M, int N, int K, int* tile, int* splits) {
       if (s > 1) us += 4.0 + (double)M * N * 4.0 * (s + 1) / 4e6;
       if (us < best) {
         best = us;
+        groups = tiles * s;
         *tile = t;
         *splits = s;
       }
     }
   }
-  return best;
+  const int steps = ceil_div(ceil_div(K, 32), *splits);
+  const double two = 5.9 + 0.52 * steps, one = 2.0 + 0.47 * steps;
+  const double last = groups % 512 > 256 ? two : groups % 512 > 0 ? one : 0.0;
+  return (*tile == 8 ? (double)((groups + 255) / 256) * (12.8 + 0.82 * steps) : (double)(groups / 512) * two + last) +
+         (*splits > 1 ? 3.3 + (double)M * N * 4.0 * (*splits + 1) / 10e6 : 0.0);
 }
 
 namespace {
 
-// decoding (2.5 bytes an element at the copy rate), and the GEMM of an [M, n] result over k
+// decoding (2.5 bytes an element), and the GEMM of an [M, n] result over k
 double decoded_us(int M, int n, int k, int64_t weight) {
   int tile, splits;
-  return 5.0 + (double)weight * 0.375e-6 + mx_gemm_plan(M, n, k, &tile, &splits);
+  return 5.7 + (double)weight * 0.375e-6 + mx_gemm_plan(M, n, k, &tile, &splits);
 }
 
-// 128-column tiles of 128 or 64 rows (*mi 4 or 2): a stage takes `one128` us in the one 128-row workgroup that fits a CU,
-// `one64` in a 64-row one alone and `two64` in two
-double big_us(int M, int cols, int stages, double one128, double one64, double two64, int* mi) {
+struct Price {
+  double start, round, stage;
+  double rounds(double n, int stages) const { return n * (round + stage * stages); }
+};
+
+// 128-column tiles of 128 rows (*mi 4), one workgroup a CU, or of 64 rows (*mi 2), one (`one`) or two (`two`)
+double big_us(int M, int cols, int stages, const Price& p128, double lone, const Price& one, const Price& two, int* mi) {
   const double w4 = (double)ceil_div(M, 128) * ceil_div(cols, 128) / 256.0, w2 = (double)ceil_div(M, 64) * ceil_div(cols, 128) / 256.0;
-  const double last = w2 - 2 * std::floor(w2 / 2);
-  const double r4 = one128 * (w4 <= 1 ? 0.93 : std::ceil(w4));  // (a lone round runs a little faster)
-  const double r2 = two64 * std::floor(w2 / 2) + (last > 1 ? one64 + 0.8 * (two64 - one64) : last > 0 ? one64 : 0.0);
+  const double full = std::floor(w2 / 2), last = w2 - 2 * full;
+  const double r4 = p128.start + p128.rounds(w4 <= 1 ? lone : std::ceil(w4), stages);  // (a lone round runs a little faster)
+  const double o = one.rounds(1, stages), t = two.rounds(1, stages);
+  const double r2 = one.start + full * t + (last > 1 ? o + 0.8 * (t - o) : last > 0 ? o : 0.0);
   *mi = r2 < r4 ? 2 : 4;
-  return 4.0 + std::min(r2, r4) * stages;
+  return std::min(r2, r4);
 }
 
 // joining the pieces' products, which the 128-column tiles need not do
 double join_us(int M, int cols, int pieces) { return pieces > 1 ? 2.5 + (double)M * cols * (4 * pieces + 4) / 3.5e6 : 0.0; }
 
+int64_t rounds_of(int rows, int row_tile, int cols, int col_tile) {
+  return ((int64_t)ceil_div(rows, row_tile) * ceil_div(cols, col_tile) + 255) / 256;
+}
+
 }  // namespace
 
 void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
-  // a round's time is a + b * groups; two or more workgroups a CU (whole = false) fill its rounds evenly
   static const struct {
     int mt, nt;
-    double a, b;
-    bool whole;
-  } kTiles[] = {{2, 4, 1.07, 0.217, true}, {2, 2, 0.6, 0.14, true}, {1, 4, 0.2, 0.1625, true}, {1, 2, 0.23, 0.096, false},
-                {1, 1, 0.2, 0.07, false}};
+    Price p;  // a stage: a group of four blocks, over the waves that share it
+  } kTiles[] = {{2, 4, {1.1, 2.4, 0.185}}, {2, 2, {1.5, 1.75, 0.12}}, {1, 4, {1.5, 1.65, 0.131}}, {1, 2, {2.8, 0.43, 0.0736}},
+                {1, 1, {2.7, 0.43, 0.051}}};
   const int K = 32 * nb, rows = pieces * M;
   const double join = join_us(M, N, pieces);
   double best = 1e30;
   for (const auto& t : kTiles) {
     if (!lds) break;
-    const double w = (double)ceil_div(rows, 16 * t.mt) * ceil_div(N, 16 * t.nt) / 256.0;
-    const double us = join + 2.5 + (t.a + t.b * (nb / 4)) * std::max(1.0, t.whole ? std::ceil(w) : w);
+    const double us = join + t.p.start + t.p.rounds((double)rounds_of(rows, 16 * t.mt, N, 16 * t.nt), nb / 4);
     if (us < best) {
       best = us;
       *mt = t.mt + kMxLds;
@@ -1231,31 +1248,39 @@ void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
     *nt = wide ? 4 : 1;
     best = join + 2.5 + 2.0 * rows * N * K / 250e6;
   }
-  int mi;
-  if (lds && big_us(M, N, nb / 4 * pieces, 1.1, 0.63, 1.17, &mi) < best) {
-    best = big_us(M, N, nb / 4 * pieces, 1.1, 0.63, 1.17, &mi);
-    *mt = kMxBig + mi;
-    *nt = kBigCols / 16;
+  if (lds) {
+    int mi;
+    const double us = big_us(M, N, nb / 4 * pieces, {0.6, 4.0, 0.91}, 0.94, {3.4, 0.25, 0.56}, {0.0, 2.5, 0.98}, &mi);
+    if (us < best) {
+      best = us;
+      *mt = kMxBig + mi;
+      *nt = kBigCols / 16;
+    }
   }
   if (join + decoded_us(rows, N, K, (int64_t)N * K) < best) *mt = *nt = 0;
 }
 
 void mx_nn_plan(int M, int N, int nb, int pieces, bool lds, int* mt) {
-  const int K = 32 * nb, all = pieces * M;
+  const int K = 32 * nb, all = pieces * M, stages = ceil_div(N, 128);
   const double join = join_us(M, K, pieces);
-  const bool ring = lds && N >= 1024 && N % 128 == 0;  // else the direct product is as fast, and activations need no padding
-  const int rows = ring && (int64_t)ceil_div(all, 16) * ceil_div(nb, 4) > 256 ? 2 : 1;
-  const int64_t rounds = (ceil_div(all, 16 * rows) * (int64_t)ceil_div(nb, 4) + 255) / 256;
-  double best = join + 2.5 + rounds * (ring ? 1.0 + (rows == 2 ? 0.48 : 0.36) * N / 128 : 0.5 + 0.6 * N / 128);
-  *mt = rows + (ring ? kMxLds : 0);
-  int mi;
+  // what goes through LDS takes whole stages; pieces are written padded, other activations have to be copied for it
   const double padding = pieces == 1 && N % 128 != 0 ? 2.5 + (double)M * N * 4 / 4.5e6 : 0.0;
-  const double big = padding + big_us(M, K, ceil_div(N, 128) * pieces, 1.13, 0.68, 1.28, &mi);
-  if (lds && big < best) {
-    best = big;
-    *mt = kMxBig + mi;
+  double best = join + 3.2 + (double)rounds_of(all, 16, K, 128) * std::max(0.1, 0.5 * N / 128 - 0.4);
+  *mt = 1;
+  auto take = [&](double us, int variant) {
+    if (us < best) {
+      best = us;
+      *mt = variant;
+    }
+  };
+  if (lds) {
+    take(join + padding + 0.8 + Price{0.0, 3.15, 0.332}.rounds((double)rounds_of(all, 16, K, 128), stages), 1 + kMxLds);
+    take(join + padding + 0.8 + Price{0.0, 4.1, 0.369}.rounds((double)rounds_of(all, 32, K, 128), stages), 2 + kMxLds);
+    int mi;
+    const double us = big_us(M, K, stages * pieces, {1.0, 5.0, 0.944}, 0.965, {4.2, 0.0, 0.675}, {0.0, 2.7, 1.13}, &mi);
+    take(padding + us, kMxBig + mi);
   }
-  if (join + decoded_us(all, K, N, (int64_t)N * K) < best) *mt = 0;
+  take(join + decoded_us(all, K, N, (int64_t)N * K), 0);
 }
 
 hipError_t mx_nt(const void* x, const uint8_t* codes, const uint8_t* scales, int M, int N, int nb, const float* bias,
