@@ -124,3 +124,11 @@ def test_a_weight_loaded_before_the_backward_is_noticed():
         y.sum().backward()
     z.sum().backward()
     assert x.grad is not None
+
+
+def test_a_weight_quantised_in_inference_mode_trains():
+    with torch.inference_mode():
+        w = quantize_mxfp4(torch.randn(8, 64))
+    x = torch.randn(3, 64, requires_grad=True)
+    mxfp4_linear(x, w).sum().backward()
+    torch.testing.assert_close(x.grad, w.dequantize(torch.float32).sum(0).expand(3, 64), atol=1e-5, rtol=1e-5)
