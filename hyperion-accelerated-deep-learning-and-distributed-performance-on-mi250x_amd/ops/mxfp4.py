@@ -201,6 +201,8 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Tensor, bias: Optional[torch.Tens
 class MXFP4Linear(nn.Module):
     """A linear layer whose weight is frozen in 4 bits (buffers ``weight_codes`` / ``weight_scales``)."""
 
+    frozen_buffers = ("weight_codes", "weight_scales")  # data parallelism need not keep them in step
+
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None):
         super().__init__()
         self.in_features, self.out_features = in_features, out_features

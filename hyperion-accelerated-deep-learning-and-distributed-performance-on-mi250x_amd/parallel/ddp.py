@@ -361,14 +361,23 @@ class DistributedDataParallel(nn.Module):
         finally:
             self._sync = prev
 
+    def _live_buffers(self):
+        """The buffers that training changes: a module names those it never does (a frozen 4-bit weight's codes) in
+        ``frozen_buffers``.  They are the same on every rank from the constructor on."""
+        for m in self.module.modules():
+            frozen = getattr(m, "frozen_buffers", ())
+            for name, b in m.named_buffers(recurse=False):
+                if name not in frozen and b.numel() > 0:
+                    yield b
+
     def sync_buffers(self) -> None:
         """Rank 0's buffers (BN running statistics) to every rank, in place (K5)."""
-        bufs = [b for b in self.module.buffers() if b.numel() > 0]
+        bufs = list(dict.fromkeys(self._live_buffers()))  # (a shared one once)
         if bufs:
             _flat_broadcast(bufs, 0, self.process_group)
 
     def has_buffers(self) -> bool:
-        return any(b.numel() > 0 for b in self.module.buffers())
+        return next(self._live_buffers(), None) is not None
 
     def forward(self, *args, **kwargs):
         if self.world > 1 and self.broadcast_buffers and self.has_buffers():

@@ -178,3 +178,41 @@ def check_one_rounding(dev, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_adapter_is_added_with_one_rounding(dtype):
     check_one_rounding("cpu", dtype)
+
+
+def _ddp_on_a_4_bit_base(rank, world):
+    from hyperion.parallel import DDP, ddp
+
+    m = build("cpu", torch.float32, seed=rank)
+    m.register_buffer("running", torch.full((3,), float(rank)))
+    sent = []
+    flat_broadcast = ddp._flat_broadcast
+
+    def spy(ts, *args):
+        sent.append(sum(t.numel() * t.element_size() for t in ts))
+        flat_broadcast(ts, *args)
+
+    ddp._flat_broadcast = spy
+    d = DDP(m)
+    ids, mask, _, _ = batch("cpu")
+    m.running += rank
+    first = d(ids, mask, return_logits=True).logits
+    second = d(ids.flip(1), mask, return_logits=True).logits  # before the first one's backward
+    with d.no_sync():
+        first.square().mean().backward()
+    second.square().mean().backward()
+    codes = [b.clone() for n, b in m.named_buffers() if n.endswith(("weight_codes", "weight_scales"))]
+    return {"sent": sent, "codes": codes, "running": m.running.clone(),
+            "grads": [p.grad.clone() for p in m.parameters() if p.grad is not None]}
+
+
+def test_ddp_broadcasts_a_4_bit_base_once():
+    from dist_utils import run_world
+
+    res = run_world(_ddp_on_a_4_bit_base, 2)
+    a, b = res[0], res[1]
+    whole = sum(c.numel() for c in a["codes"])
+    assert len(a["codes"]) == 2 * 14 and all(torch.equal(x, y) for x, y in zip(a["codes"], b["codes"]))
+    assert a["sent"][0] > whole and a["sent"][1:] == [12, 12]  # then the running statistics alone
+    assert torch.equal(a["running"], torch.zeros(3)) and torch.equal(b["running"], torch.zeros(3))
+    assert len(a["grads"]) > 0 and all(torch.equal(x, y) for x, y in zip(a["grads"], b["grads"]))
