@@ -158,14 +158,14 @@ template <typename T>
 __global__ __launch_bounds__(kQThreads) void mx_join_k(const float* __restrict__ part, int P, int64_t rows, int cols,
                                                        int64_t pitch, const float* __restrict__ bias,
                                                        T* __restrict__ y) {
-  const int64_t i = (int64_t)blockIdx.x * kQThreads + threadIdx.x;
-  if (i >= rows * cols) return;
-  const int64_t row = i / cols;
-  const int c = (int)(i - row * cols);
-  float s = 0.f;
-  for (int p = P - 1; p >= 0; --p) s += part[((int64_t)p * rows + row) * pitch + c];  // the small pieces first
-  if (bias) s += bias[c];
-  st1<T>(y + i, s);
+  for (int64_t i = (int64_t)blockIdx.x * kQThreads + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * kQThreads) {
+    const int64_t row = i / cols;
+    const int c = (int)(i - row * cols);
+    float s = 0.f;
+    for (int p = P - 1; p >= 0; --p) s += part[((int64_t)p * rows + row) * pitch + c];  // the small pieces first
+    if (bias) s += bias[c];
+    st1<T>(y + i, s);
+  }
 }
 
 // ---- activations times a 4-bit weight, decoded on the way to the matrix instructions ---------------------
@@ -1101,9 +1101,8 @@ hipError_t mx_pieces(int dtype, const void* x, int64_t ld, int64_t rows, int col
 
 hipError_t mx_join(int dtype, const float* part, int pieces, int64_t rows, int cols, int64_t pitch, const float* bias,
                    void* y, hipStream_t stream) {
-  const int64_t grid = (rows * cols + kQThreads - 1) / kQThreads;
+  const int64_t grid = std::min(kMxGridMax - 1, (rows * cols + kQThreads - 1) / kQThreads);
   if (grid == 0) return hipSuccess;
-  if (grid >= kMxGridMax) return hipErrorInvalidValue;
   HYP_DISPATCH_FLOAT(dtype, T, {
     hipLaunchKernelGGL((mx_join_k<T>), dim3(grid), dim3(kQThreads), 0, stream, part, pieces, rows, cols, pitch, bias,
                        static_cast<T*>(y));

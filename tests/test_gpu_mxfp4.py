@@ -232,3 +232,19 @@ def test_a_weight_loaded_before_the_backward_is_noticed():
         y.sum().backward()
     z.sum().backward()
     assert x.grad is not None
+
+
+def test_outputs_of_more_than_2_32_elements():
+    # the pieces' products of fp32 activations, joined: rows on both sides of element 2^32
+    M, N, K = 1 << 19, 8200, 32
+    g = torch.Generator().manual_seed(8)
+    w = quantize_mxfp4(torch.randn(N, K, generator=g).to(DEV))
+    x = torch.randn(64, K, generator=g).to(DEV).repeat(M // 64, 1)
+    y = mxfp4_linear(x, w)
+    W = decoded(w.codes, w.scales, K).to(DEV)
+    want = x[:64].double() @ W.t()
+    bound = product_bound(x[:64].double(), W.t(), torch.float32)
+    at = (1 << 32) // N // 64 * 64
+    for r in (0, at - 64, at, at + 64, M - 64):
+        assert ((y[r:r + 64].double() - want).abs() <= bound).all(), r
+    assert bool((y.view(-1, 64, N) == y[:64]).all())
