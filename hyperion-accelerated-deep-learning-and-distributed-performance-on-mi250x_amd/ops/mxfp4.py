@@ -152,21 +152,22 @@ class _MXLinearFn(torch.autograd.Function):
         else:
             y = x.float() @ w._rows(torch.float32, K).t()
             y = (y if bias is None else y + bias.float()).to(x.dtype)
-        if w.codes.is_inference() or w.scales.is_inference():  # (these have no version to check, and cannot be saved)
-            ctx.weight = w.codes, w.scales
-        else:
+        if ctx.needs_input_grad[0]:
             ctx.weight = None
-            ctx.save_for_backward(w.codes, w.scales)  # (a weight loaded before the backward is noticed there)
+            if w.codes.is_inference() or w.scales.is_inference():  # (these have no version to check, and cannot be saved)
+                ctx.weight = w.codes, w.scales
+            else:
+                ctx.save_for_backward(w.codes, w.scales)  # (a weight loaded before the backward is noticed there)
         ctx.wshape, ctx.native, ctx.xshape, ctx.bdtype = w.shape, native, x.shape, None if bias is None else bias.dtype
         return y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        codes, scales = ctx.weight or ctx.saved_tensors
         N, K = ctx.wshape
         dx = db = None
         if ctx.needs_input_grad[0]:
+            codes, scales = ctx.weight or ctx.saved_tensors
             if dy.numel() == 0 or K == 0:
                 dx = dy.new_zeros(ctx.xshape)
             elif ctx.native:
