@@ -17,12 +17,13 @@
 // formula, whatever the instructions' rounding.  The fp64 operations are those of the PyTorch path, one by
 // one and uncontracted, so that scales and codes are the same bits on CPU and GPU (0.9 S + 0.1 g is
 // often exactly halfway between two fp32 numbers, where a fused product would round the other way).
-// The parameter's update uses the uncoded moments, in fp32.
+// The parameter's update uses the uncoded moments, in fp32 and with the reciprocal and square root instructions (1 ulp
+// each); the PyTorch path computes it in fp64, so that parameters agree to a few roundings, not bit for bit.
 //
 // A half wave holds one block, 8 elements a lane; the block's maxima meet over the 32 lanes by lane
 // exchanges in registers.  Per element: gradient 2 or 4 bytes, fp32 parameter 4 + 4 (+ 2 its bf16 / fp16
-// copy), codes 2 + 2, scales 16 / 256.  Measured (MI355X): 180M bf16 parameters with masters 614 us (4.7 TB/s; a large copy
-// reaches 5.1), 16.8M in 256 tensors 58 us, 6.8M fp32 in 52 tensors 28 us.  About 80 VALU slots an element keep the
+// copy), codes 2 + 2, scales 16 / 256.  Measured (MI355X): 180M bf16 parameters with masters 588 us (4.9 TB/s; a large copy
+// reaches 5.1), 16.8M in 256 tensors 64 us, 6.8M fp32 in 52 tensors 28 us.  About 80 VALU slots an element keep the
 // lanes nearly as busy as HBM; accesses of the masters past the caches gained 2% of the first, lost 7% of the second.
 #include "hyp_common.h"
 #include "hyp_kernels.h"

@@ -493,9 +493,10 @@ __global__ __launch_bounds__(kLdsWaves * 64) void mx_nt_lds_k(const MxArgs a) {
 // decoded fragment meets MI fragments of activations.  Waves 4 h + 2 i + j own the i-th half of the rows and the j-th of
 // the columns for half h of every block's elements: two waves a SIMD (one alone issues at half rate), whose
 // sums meet in LDS.  2048 x 11008 x 4096 in 185 us in 64-row tiles, 197 in 128-row ones (1.0 PFLOP/s; decoded
-// weight and tiled GEMM 248), 450 x 4096 x 4096 in 23 us against 34 in 32-row tiles.  Halves a barrier apart (one multiplies while the other
-// reads) were slower, 37.6 against 34.6 us at 512 rows, and so was every wave bringing its own scales (42 against 36 us at
-// 700 rows in 64-row tiles).  The images are those above.  x holds P pieces [M, 32 nb] whose sum the activations are: the
+// weight and tiled GEMM 248), 450 x 4096 x 4096 in 23 us against 34 in 32-row tiles.  At 1024 x 4096 x 4096 the matrix pipe works
+// 43 % of the time, LDS 25 %, and waves wait 36 %.  Halves a barrier apart (one multiplies while the other
+// reads) were slower, 37.6 against 34.6 us for one round of 128-row tiles, and so was every wave bringing its own scales
+// (42 against 36 us at 700 rows in 64-row tiles).  The images are those above.  x holds P pieces [M, 32 nb] whose sum the activations are: the
 // reduction runs over the weight once for each, the smallest first, into the same fp32 sums.
 constexpr int kBigStages = 3, kBigCols = 128;
 
@@ -747,8 +748,9 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_nn_k(const MxArgs a) {
 // stage.  A workgroup owns 16 MT rows and 128 columns; the waves split the reduction and each fills a ring of its own as
 // above.  A lane reads 8 elements (4 bytes) of each of 8 weight rows, decodes them under each row's own scale
 // and transposes the 8 x 8 in registers (v_perm), which gives the fragments of columns 8 (l & 15) + c, c = 0..7:
-// no transposed copy of the weight, and 32 consecutive bytes of the partial tile a lane.  The decoding, about
-// 80 instructions for 32 rows, is what bounds it up to 32 rows of x.
+// no transposed copy of the weight, and 32 consecutive bytes of the partial tile a lane.  Every workgroup
+// walks all of the weight's rows, 0.33 us for 128 of them: up to 16 rows of x over 4096 columns are 32 workgroups on 256 CUs and
+// take one walk's time (14 us for 4096 weight rows), and 128 rows of x (17 us) decode each strip eight times.
 // Images: activations as above with h(r) = r; weight rows 8 g + r of every 32 at place 4 r + g, 64 bytes each, so
 // that the four lane groups read 256 consecutive bytes; scales [128 rows] of 4 bytes.
 template <int S0>

@@ -10,8 +10,8 @@
 //   dz_j = [ dlogp (delta_j - p_j) - dH p_j (q_j ln 2 + H) ] / T
 // Sums are fp32.  The forward reads every logit once, the backward reads it once and writes its
 // gradient once: HBM bounds both, with about 11 VALU slots per logit (exp2 takes 4 of them) close behind.
-// Measured, bf16: 2032 x 50257 forward 38 us (5.4 TB/s); 4064 x 50257 forward 105 us and backward 139 us, together
-// 5.0 TB/s, a large copy's rate (reading the first rows past the last-level cache, or the rows backwards in the
+// Measured, bf16: 2032 x 50257 forward 38 us (5.4 TB/s); 4064 x 50257 forward 112 us and backward 139 us under a profiler,
+// 240 together in a loop (5.1 TB/s, a large copy's rate; reading the first rows past the last-level cache, or the rows backwards in the
 // backward, changed nothing); one row with 20 alternatives 12 us, of which the launch is 3.
 //
 // Rows start at any element (V = 50257 rows of 2-byte logits are 2-byte aligned).  The forward reads the
