@@ -548,7 +548,7 @@ std::vector<at::Tensor> bn_bwd_dx_wgrad(const at::Tensor& dz, const at::Tensor& 
 namespace {
 int skinny_splits(int M, int N, int Kred, int bm, int bn, int64_t splits_req) {
   if (splits_req > 0) return (int)splits_req;
-  const int tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+  const int tiles = std::max(1, ((M + bm - 1) / bm) * ((N + bn - 1) / bn));  // (no rows: the launch refuses them)
   const int nk = Kred / 64;
   int sp = (600 + tiles - 1) / tiles;
   return std::max(1, std::min(sp, nk / 4));

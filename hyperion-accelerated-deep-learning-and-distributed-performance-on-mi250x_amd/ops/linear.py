@@ -167,6 +167,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None, l
     autocast, x and w are cast to the autocast dtype first (differentiable casts, like torch's own
     autocast of ``F.linear``), so the native kernels serve the AMP trainers too.  ``link``: a
     ``ResidualLink`` on x (see :func:`arm_link`)."""
+    if x.numel() == 0:
+        return F.linear(x, w, b)  # no rows: the kernels' plans divide by their tiles
     if not (x.is_cuda and _native.use_native(x, op="linear")) or _native.plain_fp32(x):
         if _native.plain_fp32(x) and _lf32.applies(x, w):
             return _lf32.linear_f32(x, w, b)  # large fp32 GEMMs: native fp32 MFMA where it is faster

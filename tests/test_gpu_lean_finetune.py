@@ -100,3 +100,18 @@ def test_adapter_is_added_with_one_rounding(dtype):
     from test_lean_finetune_cpu import check_one_rounding
 
     check_one_rounding("cuda", dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lead", [(0,), (2, 0)])
+def test_a_layer_without_rows(lead, dtype):
+    from test_lean_finetune_cpu import check_no_rows
+
+    check_no_rows("cuda", dtype, lead)
+
+
+def test_scores_of_single_tokens():
+    m = build("cuda", torch.bfloat16)
+    ids = torch.tensor([[3], [5]], device="cuda")
+    out = m.token_logprobs(ids, ids, top_k=2)  # nothing precedes them
+    assert out.logprobs.shape == (2, 0) and out.top_ids.shape == (2, 0, 2)

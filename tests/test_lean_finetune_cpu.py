@@ -216,3 +216,17 @@ def test_ddp_broadcasts_a_4_bit_base_once():
     assert a["sent"][0] > whole and a["sent"][1:] == [12, 12]  # then the running statistics alone
     assert torch.equal(a["running"], torch.zeros(3)) and torch.equal(b["running"], torch.zeros(3))
     assert len(a["grads"]) > 0 and all(torch.equal(x, y) for x, y in zip(a["grads"], b["grads"]))
+
+
+def check_no_rows(dev, dtype, lead):
+    layer = LoRALinear(MXFP4Linear.from_linear(torch.nn.Linear(128, 64, device=dev)), r=8, dropout=0.1, dtype=dtype).train()
+    x = torch.zeros(*lead, 128, device=dev, dtype=dtype, requires_grad=True)
+    y = layer(x)
+    assert y.shape == (*lead, 64) and y.dtype == dtype
+    grads = torch.autograd.grad(y.sum(), [x, layer.lora_A["default"].weight, layer.lora_B["default"].weight])
+    assert grads[0].shape == x.shape and not grads[1].any() and not grads[2].any()
+
+
+@pytest.mark.parametrize("lead", [(0,), (2, 0)])
+def test_a_layer_without_rows(lead):
+    check_no_rows("cpu", torch.float32, lead)
