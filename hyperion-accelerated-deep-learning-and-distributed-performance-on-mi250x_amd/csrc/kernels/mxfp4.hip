@@ -1146,7 +1146,8 @@ bool mx_lds_ok(const uint8_t* scales, int nb) { return nb % 4 == 0 && reinterpre
 // a start, and for each round a part for its ends and a part for each stage of its reduction.  The prices (us) are fitted
 // to every variant's time over 28 weights (N 768 .. 11008, K 768 .. 11008) and 16 numbers of rows (1 .. 4064), bf16; within
 // 10 % for 8 shapes in 10.  Choosing by them costs 0.3 % (forward) and 0.1 % (gradient) more than the best
-// variant of each shape, on average over the 448.  Measured, us, with what was chosen:
+// variant of each shape, on average over the 448; 0.8 % and 1 % where rows are no whole groups, over 250 more (K 96 .. 4064).
+// Measured, us, with what was chosen:
 //   forward      rows   1     16    32    64    128   300   700   1500  4064    decoded: 128   700   1500  4064
 //   4096 x 4096       4.6   4.8   5.6   7.3   10.0  22    34    55    128          29    55    78    128
 //   11008 x 4096      6.8   7.1   9.4   17    23    35    69    150   366          50    133   231   368
@@ -1229,25 +1230,21 @@ void mx_nt_plan(int M, int N, int nb, int pieces, bool lds, int* mt, int* nt) {
   static const struct {
     int mt, nt;
     Price p;  // a stage: a group of four blocks, over the waves that share it
-  } kTiles[] = {{2, 4, {1.1, 2.4, 0.185}}, {2, 2, {1.5, 1.75, 0.12}}, {1, 4, {1.5, 1.65, 0.131}}, {1, 2, {2.8, 0.43, 0.0736}},
-                {1, 1, {2.7, 0.43, 0.051}}};
+  } kTiles[] = {{2 + kMxLds, 4, {1.1, 2.4, 0.185}},    {2 + kMxLds, 2, {1.5, 1.75, 0.12}}, {1 + kMxLds, 4, {1.5, 1.65, 0.131}},
+                {1 + kMxLds, 2, {2.8, 0.43, 0.0736}}, {1 + kMxLds, 1, {2.7, 0.43, 0.051}}, {2, 4, {0.95, 3.35, 0.271}},
+                {1, 1, {3.45, 0.256, 0.0755}}};
   const int K = 32 * nb, rows = pieces * M;
   const double join = join_us(M, N, pieces);
   double best = 1e30;
   for (const auto& t : kTiles) {
-    if (!lds) break;
-    const double us = join + t.p.start + t.p.rounds((double)rounds_of(rows, 16 * t.mt, N, 16 * t.nt), nb / 4);
+    if (lds != (t.mt > kMxLds)) continue;  // (where both exist, through LDS is faster)
+    const int tile = mx_rows(t.mt);
+    const double us = join + t.p.start + t.p.rounds((double)rounds_of(rows, tile, N, 16 * t.nt), ceil_div(nb, 4));
     if (us < best) {
       best = us;
-      *mt = t.mt + kMxLds;
+      *mt = t.mt;
       *nt = t.nt;
     }
-  }
-  if (!lds) {  // direct: 250 TFLOP/s in 2 x 4 tiles where they fill the chip
-    const bool wide = rows > 16 && (int64_t)ceil_div(rows, 32) * ceil_div(N, 64) >= 160;
-    *mt = wide ? 2 : 1;
-    *nt = wide ? 4 : 1;
-    best = join + 2.5 + 2.0 * rows * N * K / 250e6;
   }
   if (lds) {
     int mi;
@@ -1266,7 +1263,7 @@ void mx_nn_plan(int M, int N, int nb, int pieces, bool lds, int* mt) {
   const double join = join_us(M, K, pieces);
   // what goes through LDS takes whole stages; pieces are written padded, other activations have to be copied for it
   const double padding = pieces == 1 && N % 128 != 0 ? 2.5 + (double)M * N * 4 / 4.5e6 : 0.0;
-  double best = join + 3.2 + (double)rounds_of(all, 16, K, 128) * std::max(0.1, 0.5 * N / 128 - 0.4);
+  double best = join + 2.8 + (double)rounds_of(all, 16, K, 128) * std::max(1.2, 0.5 * N / 128);
   *mt = 1;
   auto take = [&](double us, int variant) {
     if (us < best) {
