@@ -168,8 +168,9 @@ __device__ __forceinline__ float wave_rth(float v, int r) {
 // thread, and the aligned body in batches of U loads a thread (a long read reaches 6.2 TB/s aligned, 5.2
 // at odd elements).
 // TOP: also the k most likely tokens.
-//   1. during the pass every batch's largest logit goes to LDS; with r = ceil(k / full waves), T is the
-//      smallest of the full waves' r-th largest thread maxima: at least k logits are >= T;
+//   1. during the pass every batch's largest logit goes to LDS; with r = floor(k / full waves) + 1, T is the
+//      smallest of the full waves' r-th largest thread maxima: at least k + 1 logits are >= T, so that k are above it where
+//      no two are equal;
 //   2. the batches that hold more than T (their maxima say which, nothing is read again for it) are read
 //      again, a few dozen, and their logits above T become candidates;
 //   3. if these are fewer than k, logits equal to T follow in the order of their ids: a mask's value,
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
   if (TOP) {
     full = min(W, nv / 64);  // waves whose every thread holds a piece
     if (wv < full) {
-      const float t = wave_rth(best, (a.k + full - 1) / full);
+      const float t = wave_rth(best, a.k / full + 1);
       if (lane == 0) wtop[wv] = t;
     }
     if (tid == 0) nbatch = ncand = 0;
