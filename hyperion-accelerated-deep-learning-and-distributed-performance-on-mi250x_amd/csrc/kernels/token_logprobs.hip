@@ -32,7 +32,9 @@ namespace {
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kFloor = -200.f;  // 2^-200 is 0 in fp32: a finite stand-in for -inf in products with p = 0
 constexpr int kTopCap = 1024;     // candidates of the top alternatives kept in LDS, and batches that hold them
-constexpr int kTopPrefix = 1024;  // ids looked at for logits equal to the bound
+constexpr int kTopStep = 128;     // ids looked at together for logits equal to the bound
+constexpr int kTopPrefix = 7 * kTopStep;  // .. and at most: they fit beside fewer than k above it
+static_assert(kTopPrefix + kTokenTopMax <= kTopCap, "candidates");
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at a row's own alignment
@@ -173,8 +175,8 @@ __device__ __forceinline__ float wave_rth(float v, int r) {
 //      no two are equal;
 //   2. the batches that hold more than T (their maxima say which, nothing is read again for it) are read
 //      again, a few dozen, and their logits above T become candidates;
-//   3. if these are fewer than k, logits equal to T follow in the order of their ids: a mask's value,
-//      which the first 1024 ids hold often enough;
+//   3. if these are fewer than k, logits equal to T follow in the order of their ids: those of the first 896 ids, which
+//      hold a mask's value often enough, else all of them, where the batches that hold T are few;
 //   4. every candidate writes itself to the place given by how many are larger.
 //   Where that does not serve (a NaN or +inf in the row, more candidates than fit, ties elsewhere), k sweeps
 //   over the row pick one maximum each.
@@ -295,6 +297,18 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
     const int at = atomicAdd(&ncand, 1);
     if (at < kTopCap) cand[at] = top_key(x, id);
   };
+  // the logits of batches [b0, b1) of the list that `keep` takes become candidates
+  auto take = [&](int b0, int b1, auto keep) {
+    for (int i = tid; i < (b1 - b0) * U; i += THREADS) {
+      const int b = batches[b0 + i / U], v = (b / THREADS) * (U * THREADS) + (i % U) * THREADS + b % THREADS;
+      if (v >= nv) continue;
+      float x[N];
+      Row16<T>::open(body[v], x);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (keep(x[j])) put(x[j], head + v * N + j);
+    }
+  };
   bool served = run.s == run.s;  // uniform, like every decision below
   if (served && full == 0) {  // a short row: every logit is a candidate
     for (int i = tid; i < a.V; i += THREADS) put(ld1<T>(z + i), i);
@@ -311,23 +325,35 @@ __global__ __launch_bounds__(THREADS) void token_lp_fwd_k(const LpArgs a) {
     const int nb = nbatch;
     served = nb <= kTopCap;
     if (served) {
-      for (int i = tid; i < nb * U; i += THREADS) {
-        const int b = batches[i / U], v = (b / THREADS) * (U * THREADS) + (i % U) * THREADS + b % THREADS;
-        if (v >= nv) continue;
-        float x[N];
-        Row16<T>::open(body[v], x);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (x[j] > bound) put(x[j], head + v * N + j);
-      }
+      take(0, nb, [&](float x) { return x > bound; });
       __syncthreads();
-      const bool few = ncand < a.k;
+      const int above = ncand;
       __syncthreads();
-      if (few)
-        for (int i = tid; i < min(a.V, kTopPrefix); i += THREADS) {
-          const float x = ld1<T>(z + i);
-          if (x == bound) put(x, i);
+      if (above < a.k) {
+        bool few = true;
+        for (int p0 = 0; few && p0 < min(a.V, kTopPrefix); p0 += kTopStep) {  // in order, and no more than it takes
+          const int i = p0 + tid;
+          if (tid < kTopStep && i < a.V) {
+            const float x = ld1<T>(z + i);
+            if (x == bound) put(x, i);
+          }
+          __syncthreads();
+          few = ncand < a.k;
+          __syncthreads();
         }
+        if (few) {  // the places behind the first `above` are written anew
+          if (tid == 0) ncand = above;
+          for (int i = 0; i < it; ++i)
+            if (batch_max[i * THREADS + tid] == bound) {
+              const int at = atomicAdd(&nbatch, 1);
+              if (at < kTopCap) batches[at] = i * THREADS + tid;
+            }
+          __syncthreads();
+          if (has_one && lone == bound) put(lone, one);
+          served = nbatch <= kTopCap;
+          if (served) take(0, nbatch, [&](float x) { return x == bound; });
+        }
+      }
     }
   }
   __syncthreads();

@@ -258,3 +258,55 @@ def test_longest_row():
     # rounded to bf16 (2^-8); exponents of up to 31 are rounded a few times in fp32
     assert ((got - expect).abs() <= expect.abs() * (2.0 ** -8 + 256 * 2.0 ** -24) + 2.0 ** -22 * p[2]).all()
     assert bool((g[0, :V - 2] == g[0, 0]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R", [3, 515])
+def test_ties_at_the_last_places(R, dtype):
+    """The k-th place is shared by logits anywhere in the row: behind the first ids, beside larger ones, at both ends."""
+    V, k = 30011, 20
+    g = torch.Generator().manual_seed(R)
+    z = (torch.rand(R, V, generator=g) * 4 - 8).to(dtype)
+    for r in range(R):
+        n = r % (k + 1)  # this many above the tied ones
+        at = torch.randperm(V, generator=g)[:n + 60]
+        z[r, at[:n]] = torch.linspace(2, 6, max(n, 1))[:n].to(dtype)
+        z[r, at[n:]] = 1.0
+        if r % 3 == 0:
+            z[r, V - 1] = 1.0
+        if r % 3 == 1:
+            z[r, 2000:] = torch.where(z[r, 2000:] < 0, torch.zeros((), dtype=dtype), z[r, 2000:])  # and a flood below
+        if n and r % 2:
+            z[r, (at[:n] + 1).clamp(max=V - 1)] = 1.0  # tied ones in the batches of larger ones
+    t, a = torch.full((R,), 5), torch.ones(R)
+    zd = z.to(DEV)
+    out = token_logprobs(zd, t.to(DEV), top_k=k)
+    assert torch.equal(out.top_ids.cpu(), torch.sort(z, dim=1, descending=True, stable=True)[1][:, :k])
+    compare(zd[:3], t[:3], a[:3], a[:3], k)
+
+
+@pytest.mark.parametrize("kind", ["any", "few allowed", "one of four masked"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_alternatives_do_not_sweep_ordinary_rows(kind, dtype):
+    """Twenty alternatives of ordinary rows cost little more than none: a sweep for each was 10 to 50 times that."""
+    z = torch.randn(520, 50257, device=DEV, generator=torch.Generator(DEV).manual_seed(1)) * 2.5
+    if kind == "few allowed":
+        z[:, :50250] = -math.inf
+    elif kind == "one of four masked":
+        z[:, ::4] = -math.inf
+    z = z.to(dtype)
+    t = torch.zeros(520, dtype=torch.long, device=DEV)
+
+    def time(k):
+        best = math.inf
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(4):
+                token_logprobs(z, t, top_k=k)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert time(20) < 4 * time(0)
