@@ -477,8 +477,14 @@ hipError_t token_logprobs_fwd(int dtype, const void* z, int64_t s0, int64_t s1, 
   a.k = k;
   a.top_lp = top_lp;
   a.top_id = top_id;
-  // Few rows: 1024 threads, so that one CU has a row's loads in flight at once.  Many rows: 256, eight workgroups a CU.
-  const bool wide = rows < 512 && V > 8192;
+  // 1024 threads have a long row's loads in flight at once; 256 leave room for other rows' workgroups, and their reductions
+  // and lists are shorter.  Wide where at most one row comes to a CU (256) and it is long, or, without alternatives, two.
+  // Us with 256 / 1024 threads.  None: 64 x 32000 bf16 7.2 / 6.6, 64 x 20000 bf16 5.2 / 5.7, 256 x 50257 fp32 21 / 13; 400 x 32000
+  // fp32 15.7 / 14.5, 264 x 50257 bf16 11.9 / 13.8, 700 x 50257 fp32 28.0 / 28.9.  Five alternatives: 200 x 80000 bf16 18.2 / 17.2,
+  // 256 x 32000 fp32 13.0 / 14.4, 64 x 50257 fp32 15.3 / 13.4, 264 x 50257 fp32 21.7 / 23.2, 400 x 32000 bf16 13.0 / 20.6;
+  // one x 50257 bf16 11.0 / 11.4, with 20 alternatives, of which a wave finds k / waves + 1 in turn, 12.6 / 12.3.
+  const int64_t bytes = (int64_t)V * (dtype == kF32 ? 4 : 2);
+  const bool wide = rows <= 256 ? bytes >= (k > 8 ? 100000 : k > 0 ? 150000 : 64000) : k == 0 && rows <= 512 && bytes >= 128000;
 #define HYP_LP(TH, U, TOP)                                                                                             \
   do {                                                                                                                 \
     const int its = V / (Row16<T>::N * TH * U) + 1;                                                                    \
