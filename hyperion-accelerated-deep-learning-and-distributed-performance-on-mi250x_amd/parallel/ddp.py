@@ -23,7 +23,8 @@ MI355X design:
   parameter) points at the bucket slice, so the fused optimizer reads the reduced gradient in
   place (no copy back) and its pointer table stays valid across steps;
 * ``broadcast_buffers`` reproduces the reference's per-forward BN buffer broadcast (K5); under a
-  segmented hipGraph capture it is an eager hole before the forward, so graphed steps keep it;
+  segmented hipGraph capture it is an eager hole before the forward, so graphed steps keep it
+  (buffers that a module names in ``frozen_buffers`` are broadcast by the constructor alone);
 * a segmented capture of the whole step (``train/segments.py``, used by the trainers' captured
   step) records each bucket's all-reduce and its wait as eager holes at the points where the
   eager backward issued them: replays overlap RCCL with the rest of the backward for every model;
