@@ -137,6 +137,7 @@ class FusedAdam(torch.optim.Optimizer):
         self.zero_grad_in_step = zero_grad_in_step
         self._tables = TableCache()
         self._plan8 = None  # 8-bit states: (fingerprint, launches) of the last step that ran on the kernels alone
+        self._fits8 = None  # 8-bit states: the parameters and states (fingerprint) that _check8 let pass last
         self._values8 = None  # (fingerprint, table, its key, elements, channels-last stretches) of moment_vectors
         self._step_t: Optional[torch.Tensor] = None
         self._host_step = 0
@@ -178,6 +179,8 @@ class FusedAdam(torch.optim.Optimizer):
                 loss = closure()
         if self.state_bits == 8 and self._plan8 is not None and self._replay8():
             return loss
+        if self.state_bits == 8:
+            self._check8()
         self._host_step += 1
         launches = []  # 8-bit partitions; None once one of them took the reference path
         first = next((p for g in self.param_groups for p in g["params"] if grad_of(p) is not None), None)
@@ -276,15 +279,28 @@ class FusedAdam(torch.optim.Optimizer):
             group["eps"], group["weight_decay"], bool(group["adamw"]), lr_t, self._step_t, inv_scale, self.found_inf,
             _native.DTYPE_CODE[gdt], _native.DTYPE_CODE[pdt], bool(self.zero_grad_in_step))
 
+    def _check8(self) -> None:
+        """Refuses a step whose states do not fit the parameters, before anything of it has run: the kernels trust what
+        the state says."""
+        # (one pass in C++ where they are those of the last step that fitted)
+        fingerprint = self._values_fingerprint() if self._step_t is not None else None
+        if fingerprint is not None and fingerprint == self._fits8:
+            return
+        for group in self.param_groups:
+            for p in group["params"]:
+                st = self.state.get(p)
+                if st and (st["exp_avg_q"].numel() != p.numel() or st["exp_avg_q"].device != p.device
+                           or st["channels_last"] != _channels_last(p)):
+                    if grad_of(p) is not None:
+                        raise ValueError(f"FusedAdam(state_bits=8): a parameter (now {tuple(p.shape)}, strides {p.stride()}, "
+                                         f"on {p.device}) changed its size, memory format or device after its first step")
+                    fingerprint = None  # (not of this step)
+        self._fits8 = fingerprint
+
     def _step8(self, role, gi, ps, gs, sts, inv_scale, native):
         """One partition (a parameter dtype and a gradient dtype) with 8-bit moments; the launch, or None where the
         reference path ran."""
         pdt, gdt = ps[0].dtype, gs[0].dtype
-        for p, st in zip(ps, sts):  # the kernels trust what the state says
-            if (st["exp_avg_q"].numel() != p.numel() or st["exp_avg_q"].device != p.device
-                    or st["channels_last"] != _channels_last(p)):
-                raise ValueError(f"FusedAdam(state_bits=8): a parameter (now {tuple(p.shape)}, strides {p.stride()}, on "
-                                 f"{p.device}) changed its size, memory format or device after its first step")
         tab = None
         if native and pdt in _native.DTYPE_CODE and gdt in _native.DTYPE_CODE and all(
                 p.device == self._step_t.device and _dense(p) and _dense(g) and _same_layout(p, g)
@@ -457,7 +473,7 @@ class FusedAdam(torch.optim.Optimizer):
                     # (in the parameter's layout, which the kernels take them to have)
                     self.state[p][k] = torch.empty_like(p, dtype=torch.float32).copy_(t.detach().view(p.shape))
         self._step_t = None
-        self._plan8 = self._values8 = None
+        self._plan8 = self._fits8 = self._values8 = None
         # the table cache is kept: tables a captured graph uses stay pinned; new state tensors
         # simply key new tables
 

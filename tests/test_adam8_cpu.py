@@ -256,3 +256,31 @@ def run_main_grads(dtype, dev, adamw):
 @pytest.mark.parametrize("adamw", [True, False])
 def test_fp32_gradients_of_low_precision_parameters(dtype, adamw):
     run_main_grads(dtype, "cpu", adamw)
+
+
+def check_refused_step(dev):
+    torch.manual_seed(7)
+    p, q = torch.nn.Parameter(torch.randn(300, device=dev)), torch.nn.Parameter(torch.randn(5, 7, 3, 3, device=dev))
+    opt = FusedAdamW([p, q], state_bits=8)
+    for x in (p, q):
+        x.grad = torch.randn_like(x)
+    opt.step()
+    before, saved = p.detach().clone(), copy.deepcopy(opt.state_dict())
+    q.data = q.data.contiguous(memory_format=torch.channels_last)
+    with pytest.raises(ValueError, match="memory format"):
+        opt.step()
+    assert torch.equal(p, before) and opt.state_dict()["hyperion_step"] == saved["hyperion_step"] == 1
+    for k in ("exp_avg_q", "exp_avg_sq_q", "exp_avg_scale", "exp_avg_sq_scale"):
+        assert torch.equal(opt.state[p][k], saved["state"][0][k])
+    held, q.grad = q.grad, None
+    opt.step(), opt.step()  # q takes no part
+    q.grad = held
+    with pytest.raises(ValueError, match="memory format"):
+        opt.step()
+    q.data = q.data.contiguous()
+    opt.step()
+    assert opt.state_dict()["hyperion_step"] == 4
+
+
+def test_a_refused_step_changes_nothing():
+    check_refused_step("cpu")

@@ -4,7 +4,7 @@ import torch
 
 from hyperion.ops import FusedAdam, FusedAdamW, _native, clip_grad_norm_
 
-from test_adam8_cpu import at_the_borders, check_borders, run_against_oracle, run_main_grads
+from test_adam8_cpu import at_the_borders, check_borders, check_refused_step, run_against_oracle, run_main_grads
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -286,3 +286,7 @@ def test_captured_moment_vectors():
         held.append(other)
         assert all(torch.equal(x, y) for x, y in zip(ob.moment_vectors(), want))
         ob.state[pb[0]].update(own)
+
+
+def test_a_refused_step_changes_nothing():
+    check_refused_step(DEV)
